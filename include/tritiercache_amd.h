@@ -251,6 +251,60 @@ TT_API int tt_fused_attention_decode_batched(const tt_decode_seq* seqs, const tt
                                              size_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------
+ * Queries and keys of a step: the norm of each head (RMS over head_dim, times
+ * a weight), the position rotation, and the cast to the type the caller
+ * stores, in one launch. No counterpart in the reference, whose patch runs the
+ * model file's own modules for it (src/tri_tier/integration/patch_model.py:
+ * 98-116). For a row x of one head, R = rotary_dim, p the token's position:
+ *   y = x w / sqrt(mean(x^2) + eps)   (y = x where the weight is NULL)
+ *   z[i]       = y[i] cos[p][i] - y[i + R/2] sin[p][i]                 i < R/2
+ *   z[i + R/2] = y[i + R/2] cos[p][i + R/2] + y[i] sin[p][i + R/2]
+ *   z[j]       = y[j]                                                  j >= R
+ * Values are cast only. FP32 arithmetic, each output value rounded once (to
+ * nearest even). All strides count elements; a head's channels are adjacent.
+ * The queries of token t go to row t of q_out; its keys and values to row
+ * rows[t] of k_out and v_out (row t where rows is NULL), e.g. of the sequences'
+ * FP32 tiers. */
+#define TT_DTYPE_F32 0
+#define TT_DTYPE_F16 1
+#define TT_DTYPE_BF16 2
+typedef struct tt_qk_rope {
+    const void* q;                   /* [tokens, num_q_heads, head_dim], in_dtype */
+    const void* k;                   /* [tokens, num_kv_heads, head_dim], in_dtype */
+    const void* v;                   /* likewise, or NULL (with v_out NULL) */
+    void* q_out;                     /* [tokens, num_q_heads, head_dim], out_dtype */
+    void* k_out;                     /* [out_rows, num_kv_heads, head_dim], out_dtype */
+    void* v_out;                     /* likewise, or NULL */
+    const void* q_weight;            /* [head_dim], weight_dtype; NULL = queries without a norm */
+    const void* k_weight;            /* likewise for the keys */
+    const void* cos;                 /* [table_rows, rotary_dim], table_dtype; unused with rotary_dim 0 */
+    const void* sin;
+    const int64_t* positions;        /* [tokens] row of the tables; NULL = row t. Outside them: the
+                                        token's queries and keys are NaN */
+    const int64_t* rows;             /* [tokens] row of k_out and v_out; NULL = row t. Outside
+                                        [0, out_rows), e.g. -1 for padding: not stored. Rows that occur
+                                        twice are left with pieces of either token */
+    int64_t q_token_stride, q_head_stride;
+    int64_t k_token_stride, k_head_stride;
+    int64_t v_token_stride, v_head_stride;
+    int64_t q_out_token_stride, q_out_head_stride;
+    int64_t k_out_token_stride, k_out_head_stride;
+    int64_t v_out_token_stride, v_out_head_stride;
+    int64_t table_rows, table_stride;
+    int64_t out_rows;
+    int32_t tokens, num_q_heads, num_kv_heads;
+    int32_t head_dim;                /* a multiple of 16 of at most 256 */
+    int32_t rotary_dim;              /* a multiple of 16 of at most head_dim; 0 = no rotation */
+    float eps;
+    int32_t in_dtype, out_dtype, weight_dtype, table_dtype; /* TT_DTYPE_* */
+} tt_qk_rope;
+
+/* `args` (host memory) is read by the call only. An output may be its input
+ * (same address, type and strides, rows NULL); apart from that outputs must not
+ * overlap inputs or each other. No allocation, one kernel. */
+TT_API int tt_qk_norm_rope(const tt_qk_rope* args, void* stream);
+
+/* ---------------------------------------------------------------------------
  * Engine: replaces _C.TriTierCacheEngine (bindings.cpp:384-626, class
  * csrc/include/cache_engine.h:10-123, csrc/cache_engine.cpp). All tier buffers
  * and counters live in device memory; a step enqueues its kernels without a

@@ -36,6 +36,7 @@ __all__ = [
     "quantize_v_block",
     "dequantize_k",
     "dequantize_v",
+    "qk_norm_rope",
     "device_count",
     "version",
 ]
@@ -347,6 +348,117 @@ def dequantize_v(packed, scale, zero, out, total_tokens, num_heads, head_dim, pb
     o = st.ptr(out, "out", n * H * D * 4, writable=True)
     _lib.check(_L.tt_dequantize_v(p, s, z, o, n, H, D, int(fp16), _stream()), "dequantize_v")
     st.finish()
+
+
+_DTYPES = {torch.float32: _lib.TT_DTYPE_F32, torch.float16: _lib.TT_DTYPE_F16, torch.bfloat16: _lib.TT_DTYPE_BF16}
+
+
+def _rows(t, name: str, heads=None, like=None) -> torch.Tensor:
+    """A ROCm tensor [tokens, heads, head_dim] whose channels are adjacent (other strides are free)."""
+    if not isinstance(t, torch.Tensor) or t.dim() != 3:
+        raise ValueError(f"Argument '{name}' must be a tensor [tokens, heads, head_dim].")
+    if t.dtype not in _DTYPES:
+        raise ValueError(f"Argument '{name}' must be float32, float16 or bfloat16, got {t.dtype}.")
+    if t.shape[2] > 1 and t.numel() and t.stride(2) != 1:
+        raise ValueError(f"Argument '{name}' must have adjacent channels (stride 1 in its last dimension).")
+    if like is not None and (t.dtype != like.dtype or t.shape[2] != like.shape[2]):
+        raise ValueError(f"Argument '{name}' must have the type and head_dim of its kind: {like.dtype}, {like.shape[2]}.")
+    if heads is not None and t.shape[1] != heads:
+        raise ValueError(f"Argument '{name}' must have {heads} heads, got {t.shape[1]}.")
+    return t
+
+
+def qk_norm_rope(q, k, v=None, cos=None, sin=None, positions=None, q_weight=None, k_weight=None, eps=1e-6,
+                 out_dtype=None, rows=None, q_out=None, k_out=None, v_out=None):
+    """The norm of each query and key head, the position rotation and the cast, in one launch; no
+    counterpart in the reference (its patch runs the model file's modules, patch_model.py:98-116).
+
+    q [tokens, num_q_heads, head_dim], k and v [tokens, num_kv_heads, head_dim] (v may be None): ROCm tensors of one
+    type, any strides with adjacent channels (views of a joint projection, transposed ones). cos, sin [table rows,
+    rotary_dim]: a multiple of 16 channels is rotated, the first half of them against the second (rotate-half),
+    the rest passes; None: no rotation. positions [tokens] int64: each token's row of the tables (None: row t; a position outside them makes
+    the token's queries and keys NaN). q_weight, k_weight [head_dim]: weights of the RMS norms, None for no norm.
+    rows [tokens] int64: the row of k_out and v_out that takes the token's keys and values (None: row t; -1 or any
+    row that is not there: not stored). Outputs that are not given are allocated in out_dtype (q's type where that is None); with
+    rows, k_out and v_out are the caller's. Returns (q_out, k_out, v_out or None)."""
+    q = _rows(q, "q")
+    tokens, hq, d = q.shape
+    k = _rows(k, "k", like=q)
+    hkv = k.shape[1]
+    ins = {"q": q, "k": k}
+    if v is not None:
+        ins["v"] = _rows(v, "v", hkv, q)
+    for name, x in ins.items():
+        if x.shape[0] != tokens:
+            raise ValueError(f"Argument '{name}' must have {tokens} tokens, got {x.shape[0]}.")
+    if (cos is None) != (sin is None):
+        raise ValueError("cos and sin must both be given or both be None.")
+    if v is None and v_out is not None:
+        raise ValueError("v_out without v.")
+    small = {"cos": cos, "sin": sin, "positions": positions, "rows": rows, "q_weight": q_weight, "k_weight": k_weight}
+    for name, x in small.items():
+        if x is not None and not isinstance(x, torch.Tensor):
+            raise ValueError(f"Argument '{name}' must be a tensor.")
+    rot = 0
+    if cos is not None:
+        if cos.dim() != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.dtype not in _DTYPES:
+            raise ValueError("cos and sin must be [table rows, rotary_dim] of one type: float32, float16 or bfloat16.")
+        rot = cos.shape[1]
+        if cos.stride() != sin.stride() or (rot > 1 and cos.stride(1) != 1):
+            raise ValueError("cos and sin must have the same strides and adjacent channels.")
+    for name in ("positions", "rows"):
+        x = small[name]
+        if x is not None and (x.dtype != torch.int64 or x.shape != (tokens,) or not x.is_contiguous()):
+            raise ValueError(f"Argument '{name}' must be a contiguous int64 tensor [{tokens}].")
+    wdt = {x.dtype for x in (q_weight, k_weight) if x is not None}
+    for name in ("q_weight", "k_weight"):
+        x = small[name]
+        if x is not None and (x.dtype not in _DTYPES or x.shape != (d,) or not x.is_contiguous() or len(wdt) > 1):
+            raise ValueError("q_weight and k_weight must be contiguous [head_dim] tensors of one type.")
+    if rows is not None and (k_out is None or (v is not None and v_out is None)):
+        raise ValueError("with rows, k_out and v_out are the caller's tensors.")
+    _require_gpu()
+    odt = out_dtype
+    if odt is None:
+        given = [x for x in (q_out, k_out, v_out) if x is not None]
+        odt = given[0].dtype if given else q.dtype
+    if odt not in _DTYPES:
+        raise ValueError(f"out_dtype must be float32, float16 or bfloat16, got {odt}.")
+    outs = {}
+    for name, x, h in (("q_out", q_out, hq), ("k_out", k_out, hkv), ("v_out", v_out, hkv)):
+        if name == "v_out" and v is None:
+            continue
+        if x is None:
+            x = torch.empty((tokens, h, d), dtype=odt, device=q.device)
+        x = _rows(x, name, h)
+        if x.dtype != odt or x.shape[2] != d:
+            raise ValueError(f"Argument '{name}' must be {odt} with head_dim {d}.")
+        if (name == "q_out" or rows is None) and x.shape[0] < tokens:
+            raise ValueError(f"Argument '{name}' must have a row for each of the {tokens} tokens.")
+        outs[name] = x
+    if v is not None and outs["v_out"].shape[0] != outs["k_out"].shape[0]:
+        raise ValueError("k_out and v_out must have the same number of rows.")
+    tensors = {**ins, **outs, **{n: x for n, x in small.items() if x is not None}}
+    for name, x in tensors.items():
+        if not x.is_cuda or x.device != q.device:
+            raise ValueError(f"Argument '{name}' must be a ROCm tensor on the device of q.")
+    a = _lib.QkRope()
+    for name, x in tensors.items():
+        setattr(a, name, x.data_ptr() or None)
+    for name, x in {**ins, **outs}.items():
+        setattr(a, name + "_token_stride", x.stride(0))
+        setattr(a, name + "_head_stride", x.stride(1))
+    a.tokens, a.num_q_heads, a.num_kv_heads, a.head_dim, a.rotary_dim, a.eps = tokens, hq, hkv, d, rot, float(eps)
+    a.out_rows = outs["k_out"].shape[0]
+    if cos is not None:
+        a.table_rows, a.table_stride, a.table_dtype = cos.shape[0], cos.stride(0), _DTYPES[cos.dtype]
+        if cos.shape[0] == 1:
+            a.table_stride = rot
+    a.in_dtype, a.out_dtype = _DTYPES[q.dtype], _DTYPES[odt]
+    a.weight_dtype = _DTYPES[wdt.pop()] if wdt else _lib.TT_DTYPE_F32
+    with torch.cuda.device(q.device):
+        _lib.check(_L.tt_qk_norm_rope(C.byref(a), _stream()), "qk_norm_rope")
+    return outs["q_out"], outs["k_out"], outs.get("v_out")
 
 
 class _DeviceView:

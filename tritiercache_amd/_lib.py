@@ -36,6 +36,20 @@ class DecodeSeq(C.Structure):
         ("dense_count", C.c_int32), ("num_blocks", C.c_int32),
     ]
 
+class QkRope(C.Structure):
+    """tt_qk_rope: the arguments of tt_qk_norm_rope (device pointers, strides in elements)."""
+    _fields_ = ([(n, _vp) for n in ("q", "k", "v", "q_out", "k_out", "v_out", "q_weight", "k_weight", "cos", "sin",
+                                    "positions", "rows")]
+                + [(f"{n}_{s}_stride", C.c_int64) for n in ("q", "k", "v", "q_out", "k_out", "v_out")
+                   for s in ("token", "head")]
+                + [(n, C.c_int64) for n in ("table_rows", "table_stride", "out_rows")]
+                + [(n, C.c_int32) for n in ("tokens", "num_q_heads", "num_kv_heads", "head_dim", "rotary_dim")]
+                + [("eps", C.c_float)]
+                + [(n, C.c_int32) for n in ("in_dtype", "out_dtype", "weight_dtype", "table_dtype")])
+
+
+# tt_qk_rope's type numbers
+TT_DTYPE_F32, TT_DTYPE_F16, TT_DTYPE_BF16 = 0, 1, 2
 
 # name -> (restype, argtypes); mirrors include/tritiercache_amd.h
 _SIGNATURES = {
@@ -61,6 +75,7 @@ _SIGNATURES = {
                                             _vp]),
     "tt_batched_decode_workspace_bytes": (_sz, [C.POINTER(DecodeSeq), _i, _i, _i, _i, _i]),
     "tt_fused_attention_decode_batched": (_i, [C.POINTER(DecodeSeq), _vp, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "tt_qk_norm_rope": (_i, [_vp, _vp]),
     "tt_engine_create": (_i, [C.POINTER(_vp), _i, _i, _i, _i, _i, _i, _f, _f, _i, _i, C.c_char_p, _vp]),
     "tt_engine_destroy": (_i, [_vp]),
     "tt_engine_step": (_i, [_vp, _vp, _vp, _vp, _vp, _vp]),

@@ -23,6 +23,7 @@
 //                       511-540).
 #include "tt_attn.h"
 #include "tt_attn_line.h"
+#include "tt_wave.h"
 
 #include <algorithm>
 #include <atomic>
@@ -30,25 +31,6 @@
 namespace tt {
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kNegInf = -__builtin_huge_valf();
-
-template <int CTRL>
-__device__ __forceinline__ float dpp(float x) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
-}
-
-// Sum over the 16 lanes of a DPP row. Butterfly pairs (xor 1, xor 2, then the
-// half-row and row mirrors, which pair equal-valued quads / octets) so every
-// lane of the row ends with the bit-identical total.
-__device__ __forceinline__ float row_sum16(float x) {
-    x = x + dpp<0xB1>(x);   // quad_perm [1,0,3,2]
-    x = x + dpp<0x4E>(x);   // quad_perm [2,3,0,1]
-    x = x + dpp<0x141>(x);  // row_half_mirror
-    x = x + dpp<0x140>(x);  // row_mirror
-    return x;
-}
 
 template <int N>
 __device__ __forceinline__ void load_f32(const float* __restrict__ p, float (&x)[N]) {
@@ -70,14 +52,6 @@ __device__ __forceinline__ void load_f32(const float* __restrict__ p, float (&x)
     }
 }
 
-// A wave-uniform value as a scalar. Counts that come from the engine's device
-// state or from the kernel arguments would otherwise be read with one vector
-// load whose address is selected, a round trip before a workgroup knows its
-// share of the work. (With the tier pointers below: partials of 32/8 heads at
-// 32k 15.0 -> 14.2 us, at 4k 7.5 -> 7.3, head_dim 64 at 32k 11.7 -> 11.3; an
-// engine step of four layers at 4k 69.0 -> 66.4.)
-__device__ __forceinline__ int scalar(const int x) { return __builtin_amdgcn_readfirstlane(x); }
-
 // The FP32 tiers' addresses as values in scalar registers: a per-lane choice
 // between them is then a select. (Left to the compiler it becomes a load of the
 // chosen pointer from the kernel arguments, a round trip before each tile's
@@ -90,18 +64,6 @@ __device__ __forceinline__ TierPtrs tier_ptrs(const AttnInputs& in) {
     TierPtrs t{u(in.k0), u(in.k1), u(in.k2), u(in.v0), u(in.v1), u(in.v2)};
     asm("" : "+s"(t.k0), "+s"(t.k1), "+s"(t.k2), "+s"(t.v0), "+s"(t.v1), "+s"(t.v2));
     return t;
-}
-// A pointer into global memory whose origin does not tell (an integer, or read
-// from memory): without the address space in its type the accesses become flat
-// ones, which LDS waits include.
-template <typename T>
-__device__ __forceinline__ T* global_ptr(const uint64_t a) {
-    typedef __attribute__((address_space(1))) T* gptr;
-    return (T*)reinterpret_cast<gptr>(a);
-}
-template <typename T>
-__device__ __forceinline__ T* global_ptr(T* p) {
-    return global_ptr<T>(reinterpret_cast<uint64_t>(p));
 }
 __device__ __forceinline__ const float* global_f32(const uint64_t a) { return global_ptr<const float>(a); }
 

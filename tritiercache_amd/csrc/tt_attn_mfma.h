@@ -44,11 +44,6 @@
 // break that bound by more than 2^2, so the rescale of the accumulators is
 // rare.
 
-typedef _Float16 mf_h8 __attribute__((ext_vector_type(8)));
-typedef _Float16 mf_h2 __attribute__((ext_vector_type(2)));
-typedef float mf_f4 __attribute__((ext_vector_type(4)));
-typedef uint32_t mf_u4 __attribute__((ext_vector_type(4)));
-
 constexpr int kMfD = 128;       // head_dim of this path
 constexpr float kMfTau = 2.0f;  // slack of the lazy rescale, log2 units
 
@@ -110,34 +105,6 @@ struct DnLds {
     static constexpr int TOTAL = PART + 4 * GP * (2 + kMfD) * 4;
 };
 
-// max(a, b) for operands that are never NaN: one v_max_f32, without the
-// quieting of the operands that fmaxf adds for values it cannot see the origin of.
-__device__ __forceinline__ float fmax_nn(float a, float b) {
-    float r;
-    asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
-// max(|a|, |b|), likewise
-__device__ __forceinline__ float fmax_abs_nn(float a, float b) {
-    float r;
-    asm("v_max_f32_e64 %0, |%1|, |%2|" : "=v"(r) : "v"(a), "v"(b));
-    return r;
-}
-
-// Reductions over the four 16-lane rows of a wave (lanes n, n+16, n+32, n+48).
-__device__ __forceinline__ float xrow_max(float x) {
-    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = fmax_nn(__uint_as_float(s[0]), __uint_as_float(s[1]));
-    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return fmax_nn(__uint_as_float(t[0]), __uint_as_float(t[1]));
-}
-__device__ __forceinline__ float xrow_sum(float x) {
-    const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = __uint_as_float(s[0]) + __uint_as_float(s[1]);
-    const auto t = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return __uint_as_float(t[0]) + __uint_as_float(t[1]);
-}
-
 __device__ __forceinline__ float row_max16(float x) {
     x = fmaxf(x, dpp<0xB1>(x));
     x = fmaxf(x, dpp<0x4E>(x));
@@ -152,19 +119,6 @@ __device__ __forceinline__ uint32_t dpp_u32_quad1(uint32_t x) {
 }
 __device__ __forceinline__ uint32_t dpp_u32_quad2(uint32_t x) {
     return static_cast<uint32_t>(__builtin_amdgcn_mov_dpp(static_cast<int>(x), 0x4E, 0xF, 0xF, true));
-}
-
-// Orders this wave's LDS writes before its later LDS reads of other lanes'
-// data (LDS instructions of one wave execute in issue order).
-__device__ __forceinline__ void wave_lds_sync() {
-    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-    __builtin_amdgcn_wave_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-__device__ __forceinline__ mf_f4 mfma16x16x32(mf_u4 a, mf_u4 b, mf_f4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(mf_h8, a), __builtin_bit_cast(mf_h8, b), c, 0,
-                                                  0, 0);
 }
 
 // Two 2-bit codes of x at bit offsets 2k and 16 + 2k (mk selects them) ->
@@ -186,19 +140,6 @@ __device__ __forceinline__ uint32_t code_f16_centred(uint32_t x, uint32_t mk2, u
     const _Float16 c = static_cast<_Float16>(1024.0f + 3.0f * static_cast<float>(1 << (2 * k)));
     const mf_h2 off = {c, c};
     return __builtin_bit_cast(uint32_t, v - off);
-}
-
-// x - m * f16 (low / high half of h), one v_fma_mix_f32 (exact for m = 1
-// and h a rounding of x: the difference fits in f32).
-__device__ __forceinline__ float fma_mix_lo(uint32_t h, float negm, float x) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(negm), "v"(x));
-    return r;
-}
-__device__ __forceinline__ float fma_mix_hi(uint32_t h, float negm, float x) {
-    float r;
-    asm("v_fma_mix_f32 %0, %1, %2, %3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(r) : "v"(h), "v"(negm), "v"(x));
-    return r;
 }
 
 __device__ __forceinline__ uint32_t cvt_pk_f16(float x0, float x1) {
