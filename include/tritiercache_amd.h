@@ -250,6 +250,33 @@ TT_API int tt_fused_attention_decode_batched(const tt_decode_seq* seqs, const tt
                                              int k_group_size, int meta_fp16, void* workspace,
                                              size_t workspace_bytes, void* stream);
 
+/* Decode of a batch whose sequences share a prefix (a common system prompt or
+ * document): sequence i attends to the prefix's tokens and to its own, in one
+ * softmax over both; the prefix's tiers are read once for all sequences and
+ * multiplied with all their queries. No counterpart in the reference, whose
+ * callers hold the prefix in every sequence's cache (bindings.cpp:99-178).
+ *
+ * `prefix` (host memory): the tiers and counts of the shared tokens, shared by
+ * every sequence and only read; its Q and attn_output are not used and its
+ * mean_attn_weights must be NULL. `seqs`: as for the batched decode, each
+ * sequence's own tiers behind the prefix (dense_count and num_blocks may be 0);
+ * its mean_attn_weights, where given, receive the weights of its own tokens
+ * [dense_count + num_blocks * k_group_size] in that softmax. Any head_dim that
+ * is a multiple of 16 up to 256. A sequence that attends to no token at all
+ * gets zeros. Keys, values, scales and zeros of attended tokens, and queries,
+ * must be finite (a masked slot may hold anything); results are FP32-accurate. */
+TT_API size_t tt_shared_decode_workspace_bytes(const tt_decode_seq* prefix, const tt_decode_seq* seqs,
+                                               int num_seqs, int num_q_heads, int num_kv_heads,
+                                               int head_dim, int k_group_size);
+/* `prefix` and `seqs` are read by the call only; `seqs_device` as for the
+ * batched decode. The workspace must hold tt_shared_decode_workspace_bytes(...)
+ * bytes for these counts. No allocation; calls that overlap need a workspace each. */
+TT_API int tt_fused_attention_decode_shared(const tt_decode_seq* prefix, const tt_decode_seq* seqs,
+                                            const tt_decode_seq* seqs_device, int num_seqs,
+                                            int num_q_heads, int num_kv_heads, int head_dim,
+                                            int k_group_size, int meta_fp16, void* workspace,
+                                            size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------------------
  * Queries and keys of a step: the norm of each head (RMS over head_dim, times
  * a weight), the position rotation, and the cast to the type the caller

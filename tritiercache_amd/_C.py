@@ -32,6 +32,7 @@ _L = _lib.load()
 __all__ = [
     "TriTierCacheEngine",
     "fused_attention_decode",
+    "fused_attention_decode_shared",
     "quantize_k_block",
     "quantize_v_block",
     "dequantize_k",
@@ -214,6 +215,38 @@ _BATCH_FIELDS = ("Q", "dense_K", "dense_V", "dense_count", "PBS_K_Packed", "PBS_
                  "mean_attn_weights")
 
 
+def _fill_tiers(st, s, e, Hkv, D, kgs, msz):
+    """The tiers and counts of `e` (a dict with the keys of _BATCH_FIELDS) into the tt_decode_seq `s`."""
+    kvs = Hkv * D
+    W = max(kgs // 16, 1)
+    nd, nb = int(e.get("dense_count", 0)), int(e.get("num_blocks", 0))
+    if nd < 0:
+        raise ValueError("dense_count must be non-negative.")
+    if nb < 0:
+        raise ValueError("num_blocks must be non-negative.")
+    nd0, nb0 = nd == 0, nb == 0
+    s.dense_K = st.ptr(e.get("dense_K"), "dense_K", nd * kvs * 4, nullable=nd0) or None
+    s.dense_V = st.ptr(e.get("dense_V"), "dense_V", nd * kvs * 4, nullable=nd0) or None
+    s.PBS_K_Packed = st.ptr(e.get("PBS_K_Packed"), "PBS_K_Packed", nb * W * kvs * 4, nullable=nb0) or None
+    s.PBS_K_Scales = st.ptr(e.get("PBS_K_Scales"), "PBS_K_Scales", nb * kvs * msz, nullable=nb0) or None
+    s.PBS_K_Zeroes = st.ptr(e.get("PBS_K_Zeroes"), "PBS_K_Zeroes", nb * kvs * msz, nullable=nb0) or None
+    s.PBS_V_Packed = st.ptr(e.get("PBS_V_Packed"), "PBS_V_Packed", nb * kgs * Hkv * (D // 16) * 4,
+                            nullable=nb0) or None
+    s.PBS_V_Scales = st.ptr(e.get("PBS_V_Scales"), "PBS_V_Scales", nb * kgs * Hkv * msz, nullable=nb0) or None
+    s.PBS_V_Zeroes = st.ptr(e.get("PBS_V_Zeroes"), "PBS_V_Zeroes", nb * kgs * Hkv * msz, nullable=nb0) or None
+    s.PBS_token_ids = st.ptr(e.get("PBS_token_ids"), "PBS_token_ids", nb * kgs * 8, nullable=nb0) or None
+    s.dense_count, s.num_blocks = nd, nb
+
+
+def _fill_seq(st, s, e, Hq, Hkv, D, kgs, msz):
+    """One sequence of a batch: its query, tiers and outputs."""
+    s.Q = st.ptr(e.get("Q"), "Q", Hq * D * 4)
+    _fill_tiers(st, s, e, Hkv, D, kgs, msz)
+    s.attn_output = st.ptr(e.get("attn_output"), "attn_output", Hq * D * 4, writable=True)
+    s.mean_attn_weights = st.ptr(e.get("mean_attn_weights"), "mean_attn_weights",
+                                 (s.dense_count + s.num_blocks * kgs) * 4, writable=True, nullable=True) or None
+
+
 def fused_attention_decode_batched(batch, num_q_heads, num_kv_heads, head_dim, k_group_size=16,
                                    pbs_metadata_dtype="fp32"):
     """One decode step of many sequences in one split-K launch (plus one merge launch).
@@ -233,33 +266,10 @@ def fused_attention_decode_batched(batch, num_q_heads, num_kv_heads, head_dim, k
         return
     fp16 = _is_fp16(pbs_metadata_dtype, entries[0].get("PBS_K_Scales"))
     msz = 2 if fp16 else 4
-    kvs = Hkv * D
-    W = max(kgs // 16, 1)
     st = _Staging()
     seqs = (_lib.DecodeSeq * len(entries))()
-    for i, e in enumerate(entries):
-        nd, nb = int(e.get("dense_count", 0)), int(e.get("num_blocks", 0))
-        if nd < 0:
-            raise ValueError("dense_count must be non-negative.")
-        if nb < 0:
-            raise ValueError("num_blocks must be non-negative.")
-        nd0, nb0 = nd == 0, nb == 0
-        s = seqs[i]
-        s.Q = st.ptr(e.get("Q"), "Q", Hq * D * 4)
-        s.dense_K = st.ptr(e.get("dense_K"), "dense_K", nd * kvs * 4, nullable=nd0) or None
-        s.dense_V = st.ptr(e.get("dense_V"), "dense_V", nd * kvs * 4, nullable=nd0) or None
-        s.PBS_K_Packed = st.ptr(e.get("PBS_K_Packed"), "PBS_K_Packed", nb * W * kvs * 4, nullable=nb0) or None
-        s.PBS_K_Scales = st.ptr(e.get("PBS_K_Scales"), "PBS_K_Scales", nb * kvs * msz, nullable=nb0) or None
-        s.PBS_K_Zeroes = st.ptr(e.get("PBS_K_Zeroes"), "PBS_K_Zeroes", nb * kvs * msz, nullable=nb0) or None
-        s.PBS_V_Packed = st.ptr(e.get("PBS_V_Packed"), "PBS_V_Packed", nb * kgs * Hkv * (D // 16) * 4,
-                                nullable=nb0) or None
-        s.PBS_V_Scales = st.ptr(e.get("PBS_V_Scales"), "PBS_V_Scales", nb * kgs * Hkv * msz, nullable=nb0) or None
-        s.PBS_V_Zeroes = st.ptr(e.get("PBS_V_Zeroes"), "PBS_V_Zeroes", nb * kgs * Hkv * msz, nullable=nb0) or None
-        s.PBS_token_ids = st.ptr(e.get("PBS_token_ids"), "PBS_token_ids", nb * kgs * 8, nullable=nb0) or None
-        s.attn_output = st.ptr(e.get("attn_output"), "attn_output", Hq * D * 4, writable=True)
-        s.mean_attn_weights = st.ptr(e.get("mean_attn_weights"), "mean_attn_weights", (nd + nb * kgs) * 4,
-                                     writable=True, nullable=True) or None
-        s.dense_count, s.num_blocks = nd, nb
+    for s, e in zip(seqs, entries):
+        _fill_seq(st, s, e, Hq, Hkv, D, kgs, msz)
     n = len(entries)
     ws_bytes = int(_L.tt_batched_decode_workspace_bytes(seqs, n, Hq, Hkv, D, kgs))
     if ws_bytes == 0:
@@ -270,6 +280,47 @@ def fused_attention_decode_batched(batch, num_q_heads, num_kv_heads, head_dim, k
     rc = _L.tt_fused_attention_decode_batched(seqs, seqs_dev.data_ptr(), n, Hq, Hkv, D, kgs, int(fp16), ws.data_ptr(),
                                               ws_bytes, _stream())
     _lib.check(rc, "fused_attention_decode_batched")
+    st.finish()
+
+
+def fused_attention_decode_shared(prefix, batch, num_q_heads, num_kv_heads, head_dim, k_group_size=16,
+                                  pbs_metadata_dtype="fp32"):
+    """One decode step of sequences that share a prefix (a common system prompt or document): every sequence attends
+    to the prefix's tokens and its own in one softmax, and the prefix's tiers are read once for all of them. No
+    counterpart in the reference.
+
+    `prefix`: a dict with the tier keys of ``_BATCH_FIELDS`` (dense_K .. num_blocks without Q and the outputs), e.g.
+    ``TriTierCache.as_prefix()``. `batch`: the sequences as in fused_attention_decode_batched, each with its own
+    tiers behind the prefix (counts of 0 where it has none); mean_attn_weights receives the weights of its own tokens.
+    Attended keys and values and the queries must be finite."""
+    Hq, Hkv, D, kgs = int(num_q_heads), int(num_kv_heads), int(head_dim), int(k_group_size)
+    if Hq <= 0 or Hkv <= 0 or D <= 0:
+        raise ValueError("num_q_heads, num_kv_heads, and head_dim must be positive integers.")
+    pre = dict(prefix)
+    if pre.get("mean_attn_weights") is not None:
+        raise ValueError("the prefix has no mean attention weights.")
+    _require_gpu()
+    entries = [dict(e) if isinstance(e, dict) else dict(zip(_BATCH_FIELDS, e)) for e in batch]
+    if not entries:
+        return
+    scales = pre.get("PBS_K_Scales")
+    fp16 = _is_fp16(pbs_metadata_dtype, scales if scales is not None else entries[0].get("PBS_K_Scales"))
+    msz = 2 if fp16 else 4
+    st = _Staging()
+    p = _lib.DecodeSeq()
+    _fill_tiers(st, p, pre, Hkv, D, kgs, msz)
+    seqs = (_lib.DecodeSeq * len(entries))()
+    for s, e in zip(seqs, entries):
+        _fill_seq(st, s, e, Hq, Hkv, D, kgs, msz)
+    n = len(entries)
+    ws_bytes = int(_L.tt_shared_decode_workspace_bytes(C.byref(p), seqs, n, Hq, Hkv, D, kgs))
+    if ws_bytes == 0:
+        _lib.check(_lib.TT_ERR_INVALID_ARGUMENT, "fused_attention_decode_shared")
+    ws = torch.empty(ws_bytes, dtype=torch.uint8, device="cuda")
+    seqs_dev = torch.from_numpy(np.frombuffer(bytes(seqs), dtype=np.uint8).copy()).cuda()
+    rc = _L.tt_fused_attention_decode_shared(C.byref(p), seqs, seqs_dev.data_ptr(), n, Hq, Hkv, D, kgs, int(fp16),
+                                             ws.data_ptr(), ws_bytes, _stream())
+    _lib.check(rc, "fused_attention_decode_shared")
     st.finish()
 
 

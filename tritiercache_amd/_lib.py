@@ -75,6 +75,9 @@ _SIGNATURES = {
                                             _vp]),
     "tt_batched_decode_workspace_bytes": (_sz, [C.POINTER(DecodeSeq), _i, _i, _i, _i, _i]),
     "tt_fused_attention_decode_batched": (_i, [C.POINTER(DecodeSeq), _vp, _i, _i, _i, _i, _i, _i, _vp, _sz, _vp]),
+    "tt_shared_decode_workspace_bytes": (_sz, [C.POINTER(DecodeSeq), C.POINTER(DecodeSeq), _i, _i, _i, _i, _i]),
+    "tt_fused_attention_decode_shared": (_i, [C.POINTER(DecodeSeq), C.POINTER(DecodeSeq), _vp, _i, _i, _i, _i, _i, _i,
+                                              _vp, _sz, _vp]),
     "tt_qk_norm_rope": (_i, [_vp, _vp]),
     "tt_engine_create": (_i, [C.POINTER(_vp), _i, _i, _i, _i, _i, _i, _f, _f, _i, _i, C.c_char_p, _vp]),
     "tt_engine_destroy": (_i, [_vp]),

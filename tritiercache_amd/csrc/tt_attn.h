@@ -144,8 +144,13 @@ struct BatchPlan {
 };
 
 BatchPlan batch_plan(const tt_decode_seq* seqs, int nseq, int Hq, int Hkv, int D, int kgs, int meta_fp16);
+// The rest of a plan whose slot_base is filled: logits rows, mean-weight workgroups, workspace.
+void batch_layout(BatchPlan& plan, const tt_decode_seq* seqs, int Hq, int D, int kgs);
 // Enqueues the batched partials and the batched merge / mean weights.
 int batch_launch(const BatchPlan& plan, const tt_decode_seq* seqs_dev, int Hq, int Hkv, int kgs, int meta_fp16,
                  void* ws, hipStream_t stream);
+// The merge and mean weights alone, of partials of any head_dim in the plan's slots.
+int batch_finalize(const BatchPlan& plan, const tt_decode_seq* seqs_dev, int Hq, int D, int kgs, void* ws,
+                   hipStream_t stream);
 
 }  // namespace tt

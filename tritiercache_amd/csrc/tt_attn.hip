@@ -1186,7 +1186,7 @@ struct FinBatchArgs {
     const float* acc;
     const float* logits;
     float* rowstat;
-    int nseq, Hq, kgs;
+    int nseq, Hq, D, kgs;
     int msl;  // merge workgroups per (sequence, query head)
     int slot_base[kMaxBatchSeqs + 1];
     int tok_base[kMaxBatchSeqs + 1];
@@ -1197,9 +1197,9 @@ __device__ __forceinline__ FinArgs fin_batch_args(const FinBatchArgs& b, const i
     const tt_decode_seq& d = b.seqs[i];
     FinArgs a;
     a.part_ml = b.ml + static_cast<size_t>(b.slot_base[i]) * b.Hq * 2;
-    a.part_acc = b.acc + static_cast<size_t>(b.slot_base[i]) * b.Hq * kMfD;
+    a.part_acc = b.acc + static_cast<size_t>(b.slot_base[i]) * b.Hq * b.D;
     a.nsplit = b.slot_base[i + 1] - b.slot_base[i];
-    a.D = kMfD;
+    a.D = b.D;
     a.Hq = b.Hq;
     a.pair_g = 0;
     a.out = global_ptr(d.attn_output);
@@ -1765,18 +1765,14 @@ BatchPlan batch_plan(const tt_decode_seq* seqs, int nseq, int Hq, int Hkv, int D
     // (at least ~8 units of work per slot, as for one sequence).
     const long long round = std::max<long long>(1, static_cast<long long>(res.cus) * res.per_cu / heads);
     constexpr long long kBatchSlotUnits = 40;  // work units per slot below which another round does not pay
-    long long units[kMaxBatchSeqs], dunits[kMaxBatchSeqs], total = 0, mean_blocks = 0;
+    long long units[kMaxBatchSeqs], dunits[kMaxBatchSeqs], total = 0;
     for (int i = 0; i < nseq; ++i) {
         const long long pairs = (static_cast<long long>(seqs[i].num_blocks) * W + 1) / 2;
         dunits[i] = (static_cast<long long>(seqs[i].dense_count) + 15) / 16 * kDenseTileCost;
         units[i] = pairs + dunits[i];
         total += units[i];
-        if (seqs[i].mean_attn_weights)
-            mean_blocks += (static_cast<long long>(seqs[i].dense_count) + static_cast<long long>(seqs[i].num_blocks) * kgs +
-                            kMeanTokens - 1) / kMeanTokens;
     }
     const long long target = std::max<long long>(1, std::min<long long>(round, total / 8));
-    const long long per_wg = std::max<long long>(1, (mean_blocks + kMeanMaxWgs - 1) / kMeanMaxWgs);
     // Per sequence: packed slots np[i] (at least one) and FP32-tier slots
     // nd[i] (at most one per tile), sized to the work rather than rounded
     // from each sequence's fraction of it (with a few slots per sequence,
@@ -1853,28 +1849,37 @@ BatchPlan batch_plan(const tt_decode_seq* seqs, int nseq, int Hq, int Hkv, int D
     } else {
         one_cap(target);
     }
-    long long slot = 0, tok = 0, mean = 0, pk = 0, dn = 0;
     for (int i = 0; i < nseq; ++i) {
-        p.slot_base[i] = static_cast<int>(slot);
-        p.pk_base[i] = static_cast<int>(pk);
-        p.dn_base[i] = static_cast<int>(dn);
-        slot += np[i] + nd[i];
-        pk += np[i];
-        dn += nd[i];
+        p.pk_base[i + 1] = p.pk_base[i] + static_cast<int>(np[i]);
+        p.dn_base[i + 1] = p.dn_base[i] + static_cast<int>(nd[i]);
+        p.slot_base[i + 1] = p.slot_base[i] + static_cast<int>(np[i] + nd[i]);
+    }
+    batch_layout(p, seqs, Hq, D, kgs);
+    return p;
+}
+
+void batch_layout(BatchPlan& p, const tt_decode_seq* seqs, int Hq, int D, int kgs) {
+    const int nseq = p.nseq;
+    auto tokens = [&](const int i) {
+        return static_cast<long long>(seqs[i].dense_count) + static_cast<long long>(seqs[i].num_blocks) * kgs;
+    };
+    long long mean_blocks = 0;
+    for (int i = 0; i < nseq; ++i)
+        if (seqs[i].mean_attn_weights) mean_blocks += (tokens(i) + kMeanTokens - 1) / kMeanTokens;
+    const long long per_wg = std::max<long long>(1, (mean_blocks + kMeanMaxWgs - 1) / kMeanMaxWgs);
+    long long tok = 0, mean = 0;
+    for (int i = 0; i < nseq; ++i) {
         p.tok_base[i] = static_cast<int>(tok);
         p.mean_base[i] = static_cast<int>(mean);
         if (seqs[i].mean_attn_weights) {
-            const long long tub = static_cast<long long>(seqs[i].dense_count) + static_cast<long long>(seqs[i].num_blocks) * kgs;
-            tok += (tub + 3) & ~3LL;
-            mean += ((tub + kMeanTokens - 1) / kMeanTokens + per_wg - 1) / per_wg;
+            tok += (tokens(i) + 3) & ~3LL;
+            mean += ((tokens(i) + kMeanTokens - 1) / kMeanTokens + per_wg - 1) / per_wg;
         }
     }
-    p.pk_base[nseq] = static_cast<int>(pk);
-    p.dn_base[nseq] = static_cast<int>(dn);
-    p.slot_base[nseq] = static_cast<int>(slot);
     p.tok_base[nseq] = static_cast<int>(tok);
     p.mean_base[nseq] = static_cast<int>(mean);
-    p.total_slots = static_cast<int>(slot);
+    const size_t slot = static_cast<size_t>(p.slot_base[nseq]);
+    p.total_slots = p.slot_base[nseq];
     size_t off = 0;
     p.off_ml = off;
     off = align256(off + sizeof(float) * 2 * static_cast<size_t>(Hq) * slot);
@@ -1885,7 +1890,6 @@ BatchPlan batch_plan(const tt_decode_seq* seqs, int nseq, int Hq, int Hkv, int D
     p.off_logits = off;
     off = align256(off + sizeof(float) * static_cast<size_t>(Hq) * std::max<long long>(tok, 4));
     p.bytes = off;
-    return p;
 }
 
 int batch_launch(const BatchPlan& plan, const tt_decode_seq* seqs_dev, int Hq, int Hkv, int kgs, int meta_fp16,
@@ -1923,18 +1927,25 @@ int batch_launch(const BatchPlan& plan, const tt_decode_seq* seqs_dev, int Hq, i
     default: rc = launch_batched_meta<8>(b, static_cast<unsigned>(wgs), meta_fp16, stream); break;
     }
     if (rc) return rc;
+    return batch_finalize(plan, seqs_dev, Hq, kMfD, kgs, ws, stream);
+}
+
+int batch_finalize(const BatchPlan& plan, const tt_decode_seq* seqs_dev, int Hq, int D, int kgs, void* ws,
+                   hipStream_t stream) {
+    char* base = static_cast<char*>(ws);
     FinBatchArgs f;
     f.seqs = seqs_dev;
-    f.ml = b.ml;
-    f.acc = b.acc;
-    f.logits = b.logits;
+    f.ml = reinterpret_cast<const float*>(base + plan.off_ml);
+    f.acc = reinterpret_cast<const float*>(base + plan.off_acc);
+    f.logits = reinterpret_cast<const float*>(base + plan.off_logits);
     f.rowstat = reinterpret_cast<float*>(base + plan.off_rowstat);
     f.nseq = plan.nseq;
     f.Hq = Hq;
+    f.D = D;
     f.kgs = kgs;
     int max_split = 1;
     for (int i = 0; i < plan.nseq; ++i) max_split = std::max(max_split, plan.slot_base[i + 1] - plan.slot_base[i]);
-    f.msl = fin_merge_slices(kMfD, 0, max_split);
+    f.msl = fin_merge_slices(D, 0, max_split);
     std::memcpy(f.slot_base, plan.slot_base, sizeof(f.slot_base));
     std::memcpy(f.tok_base, plan.tok_base, sizeof(f.tok_base));
     std::memcpy(f.mean_base, plan.mean_base, sizeof(f.mean_base));

@@ -6,6 +6,7 @@
 // exactly when their count is zero) and adds the shape limits of the gfx950
 // kernels (GQA ratio integral, head_dim a multiple of 16 of at most 256).
 #include "tt_attn.h"
+#include "tt_shared.h"
 
 #include <algorithm>
 #include <mutex>
@@ -202,6 +203,23 @@ size_t batch_bytes(const tt_decode_seq* seqs, int num_seqs, int Hq, int Hkv, int
     for (int c0 = 0; c0 < num_seqs; c0 += kMaxBatchSeqs)
         b = std::max(b, batch_plan(seqs + c0, std::min(kMaxBatchSeqs, num_seqs - c0), Hq, Hkv, D, kgs, meta_fp16).bytes);
     return b;
+}
+
+// Validates a batch behind a shared prefix: the batch as above, the prefix as
+// a sequence without a query or outputs, and the attended tokens of each.
+int check_shared(const tt_decode_seq* prefix, const tt_decode_seq* seqs, int num_seqs, int Hq, int Hkv, int D, int kgs) {
+    if (!prefix) TT_FAIL(TT_ERR_INVALID_ARGUMENT, "Argument 'prefix' pointer address is NULL.");
+    int rc = check_batch(seqs, num_seqs, Hq, Hkv, D, kgs);
+    if (rc) return rc;
+    const void* ph = prefix;  // no query is read from the prefix: a placeholder for the shared validation
+    rc = prepare(static_cast<const float*>(ph), prefix->dense_K, prefix->dense_V, prefix->dense_count, prefix->PBS_K_Packed,
+                 prefix->PBS_K_Scales, prefix->PBS_K_Zeroes, prefix->PBS_V_Packed, prefix->PBS_V_Scales,
+                 prefix->PBS_V_Zeroes, prefix->PBS_token_ids, prefix->num_blocks, Hq, Hkv, D, kgs, 0, false, nullptr,
+                 nullptr);
+    if (rc) return rc;
+    if (prefix->mean_attn_weights)
+        TT_FAIL(TT_ERR_INVALID_ARGUMENT, "the prefix has no mean attention weights: mean_attn_weights must be NULL.");
+    return TT_OK;
 }
 
 }  // namespace
@@ -461,6 +479,41 @@ int tt_fused_attention_decode_batched(const tt_decode_seq* seqs, const tt_decode
         const BatchPlan plan = batch_plan(seqs + c0, n, Hq, Hkv, D, kgs, meta_fp16);
         rc = batch_launch(plan, seqs_device + c0, Hq, Hkv, kgs, meta_fp16, workspace, s);
         if (rc) return rc;
+    }
+    return TT_OK;
+}
+
+size_t tt_shared_decode_workspace_bytes(const tt_decode_seq* prefix, const tt_decode_seq* seqs, int num_seqs,
+                                        int num_q_heads, int num_kv_heads, int head_dim, int k_group_size) {
+    clear_error();
+    if (check_shared(prefix, seqs, num_seqs, num_q_heads, num_kv_heads, head_dim, k_group_size) != TT_OK) return 0;
+    size_t b = 256;
+    for (int c0 = 0; c0 < num_seqs; c0 += kMaxBatchSeqs)
+        b = std::max(b, shared_plan(*prefix, seqs + c0, std::min(kMaxBatchSeqs, num_seqs - c0), num_q_heads,
+                                    num_kv_heads, head_dim, k_group_size).batch.bytes);
+    return b;
+}
+
+int tt_fused_attention_decode_shared(const tt_decode_seq* prefix, const tt_decode_seq* seqs,
+                                     const tt_decode_seq* seqs_device, int num_seqs, int num_q_heads, int num_kv_heads,
+                                     int head_dim, int k_group_size, int meta_fp16, void* workspace,
+                                     size_t workspace_bytes, void* stream) {
+    clear_error();
+    const int Hq = num_q_heads, Hkv = num_kv_heads, D = head_dim, kgs = k_group_size;
+    int rc = check_shared(prefix, seqs, num_seqs, Hq, Hkv, D, kgs);
+    if (rc) return rc;
+    if (num_seqs == 0) return TT_OK;
+    if (!seqs_device) TT_FAIL(TT_ERR_INVALID_ARGUMENT, "Argument 'seqs_device' pointer address is NULL.");
+    // (chunks of kMaxBatchSeqs sequences run one after another on the stream and share the workspace)
+    for (int pass = 0; pass < 2; ++pass) {
+        for (int c0 = 0; c0 < num_seqs; c0 += kMaxBatchSeqs) {
+            const SharedPlan plan = shared_plan(*prefix, seqs + c0, std::min(kMaxBatchSeqs, num_seqs - c0), Hq, Hkv, D, kgs);
+            if (pass == 0 && (!workspace || workspace_bytes < plan.batch.bytes))
+                TT_FAIL(TT_ERR_INVALID_ARGUMENT, "workspace is NULL or smaller than tt_shared_decode_workspace_bytes().");
+            if (pass == 0) continue;
+            rc = shared_launch(plan, *prefix, seqs_device + c0, Hq, Hkv, D, kgs, meta_fp16, workspace, as_stream(stream));
+            if (rc) return rc;
+        }
     }
     return TT_OK;
 }
