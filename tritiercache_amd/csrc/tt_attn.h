@@ -149,8 +149,9 @@ void batch_layout(BatchPlan& plan, const tt_decode_seq* seqs, int Hq, int D, int
 // Enqueues the batched partials and the batched merge / mean weights.
 int batch_launch(const BatchPlan& plan, const tt_decode_seq* seqs_dev, int Hq, int Hkv, int kgs, int meta_fp16,
                  void* ws, hipStream_t stream);
-// The merge and mean weights alone, of partials of any head_dim in the plan's slots.
+// The merge and mean weights alone, of partials of any head_dim in the plan's
+// slots (`waves`: a wave per query head instead of workgroups).
 int batch_finalize(const BatchPlan& plan, const tt_decode_seq* seqs_dev, int Hq, int D, int kgs, void* ws,
-                   hipStream_t stream);
+                   hipStream_t stream, bool waves = false);
 
 }  // namespace tt

@@ -701,7 +701,12 @@ __device__ __forceinline__ void dense_body(const SplitArgs& a, const int dsplit,
 // leaves every column the logits of its own tile, and each lane runs the
 // softmax over 4 tokens rather than 8. In the PV operand the K elements
 // of the other tile are zero, which keeps the token order of the V codes.
-template <int GP, typename MetaT, bool PAIR = false>
+//
+// RANGE: K scales of any size. The coefficients are f16, so scales far from 1
+// are staged times a power of two, which the logits' factor takes back: the
+// first pair's largest scale sets it where that is below 2^-6, a larger one
+// than 2^12 raises it. Blocks without an attended slot count as zeros.
+template <int GP, typename MetaT, bool PAIR = false, bool RANGE = false>
 __device__ __forceinline__ void packed_body(const SplitArgs& a, const int split, const int kvh, const int chunk,
                                             char* lds) {
     static_assert(GP >= 1 && GP <= 8, "at most 8 query heads per workgroup");
@@ -899,6 +904,9 @@ __device__ __forceinline__ void packed_body(const SplitArgs& a, const int split,
     for (int s = 0; s < 8; ++s) acc[s] = mf_f4{0.0f, 0.0f, 0.0f, 0.0f};
     float m_run = -1.0e30f, l_run = 0.0f, pz = 0.0f;
 
+    int k_exp = 0;  // RANGE: exponent of the staged K scales
+    bool k_first = true;
+
     // Lays the fetched pair out in LDS; returns the token-validity mask.
     auto stage = [&]() -> uint32_t {
         // K: bytes tq of channels c..c+3 -> one dword per token quad.
@@ -931,8 +939,30 @@ __device__ __forceinline__ void packed_body(const SplitArgs& a, const int split,
             vt_l[vt_dword(16 * hf + 4 * g + (lane & 3), 2 * (m & 3) + (m >> 2))] = y;
         }
         float* kzd = ksz_l + (lane >> 5) * 2 * kKSZ + lk + 4 * ((lane & 31) >> 3);
-        *reinterpret_cast<float4*>(kzd) = MR::f4(ksr);
-        *reinterpret_cast<float4*>(kzd + kKSZ) = MR::f4(kzr);
+        if constexpr (RANGE) {
+            const uint32_t seen = static_cast<uint32_t>(__ballot(okv && idv != -1));
+            const bool any = (W == 2 ? seen : (lane < 32 ? seen & 0xffffu : seen >> 16)) != 0u;
+            float4 sc = MR::f4(ksr), ze = MR::f4(kzr);
+            sc = make_float4(any ? sc.x : 0.0f, any ? sc.y : 0.0f, any ? sc.z : 0.0f, any ? sc.w : 0.0f);
+            ze = make_float4(any ? ze.x : 0.0f, any ? ze.y : 0.0f, any ? ze.z : 0.0f, any ? ze.w : 0.0f);
+            float mx = fmax_nn(fmax_abs_nn(sc.x, sc.y), fmax_abs_nn(sc.z, sc.w));
+            if (__ballot(mx > __builtin_amdgcn_ldexpf(4096.0f, k_exp)) || (k_first && __ballot(mx > 0.0f))) {
+                mx = xrow_max(row_max16(mx));
+                const int e = scalar(__builtin_amdgcn_frexp_expf(mx));
+                if (e > k_exp + 12 || (k_first && e < -5)) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) crow[r] = __builtin_amdgcn_ldexpf(crow[r], e - k_exp);
+                    k_exp = e;
+                }
+                k_first = false;
+            }
+            const float f = __builtin_amdgcn_ldexpf(1.0f, -k_exp);
+            *reinterpret_cast<float4*>(kzd) = make_float4(sc.x * f, sc.y * f, sc.z * f, sc.w * f);
+            *reinterpret_cast<float4*>(kzd + kKSZ) = ze;
+        } else {
+            *reinterpret_cast<float4*>(kzd) = MR::f4(ksr);
+            *reinterpret_cast<float4*>(kzd + kKSZ) = MR::f4(kzr);
+        }
         const bool ok = okv && idv != -1;
         const int pos = 8 * ((t2 & 15) >> 2) + 4 * (t2 >> 4) + (t2 & 3);
         // lanes 32-63 hold the token's zero, lanes 0-31 its scale: the zero of

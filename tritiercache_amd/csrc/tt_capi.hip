@@ -489,8 +489,9 @@ size_t tt_shared_decode_workspace_bytes(const tt_decode_seq* prefix, const tt_de
     if (check_shared(prefix, seqs, num_seqs, num_q_heads, num_kv_heads, head_dim, k_group_size) != TT_OK) return 0;
     size_t b = 256;
     for (int c0 = 0; c0 < num_seqs; c0 += kMaxBatchSeqs)
-        b = std::max(b, shared_plan(*prefix, seqs + c0, std::min(kMaxBatchSeqs, num_seqs - c0), num_q_heads,
-                                    num_kv_heads, head_dim, k_group_size).batch.bytes);
+        for (int f = 0; f < 2; ++f)  // the larger over both metadata types
+            b = std::max(b, shared_plan(*prefix, seqs + c0, std::min(kMaxBatchSeqs, num_seqs - c0), num_q_heads,
+                                        num_kv_heads, head_dim, k_group_size, f).batch.bytes);
     return b;
 }
 
@@ -507,7 +508,8 @@ int tt_fused_attention_decode_shared(const tt_decode_seq* prefix, const tt_decod
     // (chunks of kMaxBatchSeqs sequences run one after another on the stream and share the workspace)
     for (int pass = 0; pass < 2; ++pass) {
         for (int c0 = 0; c0 < num_seqs; c0 += kMaxBatchSeqs) {
-            const SharedPlan plan = shared_plan(*prefix, seqs + c0, std::min(kMaxBatchSeqs, num_seqs - c0), Hq, Hkv, D, kgs);
+            const SharedPlan plan = shared_plan(*prefix, seqs + c0, std::min(kMaxBatchSeqs, num_seqs - c0), Hq, Hkv, D, kgs,
+                                                meta_fp16 ? 1 : 0);
             if (pass == 0 && (!workspace || workspace_bytes < plan.batch.bytes))
                 TT_FAIL(TT_ERR_INVALID_ARGUMENT, "workspace is NULL or smaller than tt_shared_decode_workspace_bytes().");
             if (pass == 0) continue;
