@@ -21,7 +21,7 @@
 // powers of two: Q by its row's largest value (to below 2^12), K and V by 16 and,
 // where a tile holds larger values than 4080 or the first one only values below
 // 1/8, by the exponent that brings them back (k_exp, v_exp; the tile is staged
-// again), P by the running reference m = max - 12 (P <= 2^14 with the slack of
+// again), P by the running reference m = max - 5 (P <= 2^14 with the slack of
 // the lazy rescale).
 #include "tt_shared.h"
 #include "tt_wave.h"
@@ -40,9 +40,11 @@ constexpr double kDenseCost = 1.5;  // an FP32 tile in packed ones
 
 constexpr int kTile = 32;           // tokens of a tile: FP32 rows or packed slots
 constexpr float kLimit = 65000.0f;  // scaled keys and values stay below this
-constexpr float kLow = 0.125f;      // a first tile of smaller keys or values is scaled up
-constexpr float kSlack = 2.0f;      // of the lazy rescale, log2 units
-constexpr float kUp = 12.0f;        // P's largest value when the reference moves, log2 units
+// P's largest value when a row's reference moves, and how much further its
+// logits may rise before it moves again, log2 units: P <= 2^14. (With 12 and 2 a
+// wave of 32 rows rescaled in every other tile.)
+constexpr float kUp = 5.0f;
+constexpr float kSlack = 9.0f;
 
 // LDS of one tile: K as [token][channel], V as [channel][token in MFMA order],
 // high and low parts (V's packed codes: one part), and of packed tiles V's
@@ -62,17 +64,14 @@ struct TileLds {
 
 constexpr int kLds = 160 * 1024;  // of a CU
 
-template <int DC, int RT, int WM, int WT>
+// Workgroups of WM waves, all on the same tile with rows of their own: two
+// tiles in LDS in turn, two waves per SIMD.
+template <int DC, int WM>
 struct Config {
-    static constexpr int WAVES = WM * WT;
-    static constexpr bool ALONE = WM == 1;  // every wave stages for itself
-    // two tiles in turn, so that staging one needs no wait for the readers of the other, where two waves per SIMD fit
-    static constexpr int NBUF = !ALONE && WT == 1 && 2 * TileLds<DC>::BYTES * 8 / WM <= kLds - 256 ? 2 : 1;
-    static constexpr int TILES = NBUF * WT;
-    static constexpr int PEAKS = ALONE ? 2 * WT : 2 * NBUF;
-    static constexpr int LDS = TILES * TileLds<DC>::BYTES + 16 * ((PEAKS + 3) / 4);
-    static constexpr int PER_CU = kLds / LDS < 8 / WAVES ? kLds / LDS : 8 / WAVES;
-    static constexpr int PER_EU = PER_CU * WAVES >= 8 ? 2 : 1;
+    static constexpr int ROWS = (DC > 4 ? 16 : 32) * WM;
+    static constexpr int LDS = 2 * TileLds<DC>::BYTES + 16;
+    static constexpr int PER_CU = kLds / LDS < 8 / WM ? kLds / LDS : 8 / WM;
+    static constexpr int PER_EU = PER_CU * WM >= 8 ? 2 : 1;
 };
 
 struct SharedArgs {
@@ -88,11 +87,29 @@ struct SharedArgs {
     int slot_base[kMaxBatchSeqs + 1];
 };
 
-// (hi, lo) of two values, both truncated: hi + lo is x to 21 bits.
-__device__ __forceinline__ uint2 parts(const float x0, const float x1) {
-    const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(x0, x1));
-    const float r0 = fma_mix_lo(hi, -1.0f, x0), r1 = fma_mix_hi(hi, -1.0f, x1);
-    return make_uint2(hi, __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1)));
+// (hi, lo) of two values, both truncated: hi + lo is x to 21 bits. `neg1` is -1
+// whose value the compiler does not know: the remainder is then one mixed fused
+// multiply-add instead of a conversion and a subtraction.
+__device__ __forceinline__ uint2 parts(const float x0, const float x1, const float neg1) {
+    const auto hi = __builtin_amdgcn_cvt_pkrtz(x0, x1);
+    const mf_h2 h = __builtin_bit_cast(mf_h2, hi);
+    const float r0 = __builtin_fmaf(static_cast<float>(h.x), neg1, x0), r1 = __builtin_fmaf(static_cast<float>(h.y), neg1, x1);
+    return make_uint2(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1)));
+}
+
+// The exponent of the scale for keys and values up to `peak` (0: not known): 16 peak 2^-e in 2^11 .. 2^12 for `below` = 8, which
+// leaves a factor of 16 for the tiles to come.
+__device__ __forceinline__ int exponent(const float peak, const int below) {
+    return peak > 0.0f ? max(scalar(__builtin_amdgcn_frexp_expf(fminf(peak, 3.0e38f))) - below, -118) : 0;
+}
+
+// The largest x (>= 0) of a wave, in every lane.
+__device__ __forceinline__ float wave_max(float x) {
+    x = fmax_nn(x, dpp<0xB1>(x));
+    x = fmax_nn(x, dpp<0x4E>(x));
+    x = fmax_nn(x, dpp<0x141>(x));
+    x = fmax_nn(x, dpp<0x140>(x));
+    return xrow_max(x);
 }
 
 __device__ __forceinline__ float half_lo(const uint32_t x) { return f16_to_f32(static_cast<uint16_t>(x & 0xffffu)); }
@@ -137,104 +154,171 @@ __device__ __forceinline__ void lds_barrier() {
     __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
 }
 
+// The largest k and v (>= 0) of a workgroup of WM waves, in every lane, through `lds`, which is free behind the next barrier.
+template <int WM>
+__device__ __forceinline__ float2 group_max(float k, float v, char* lds, const int wave, const int lane) {
+    float2* x = reinterpret_cast<float2*>(lds);
+    k = wave_max(k);
+    v = wave_max(v);
+    if (lane == 0) x[wave] = make_float2(k, v);
+    lds_barrier();
+    float2 m = x[0];
+#pragma unroll
+    for (int i = 1; i < WM; ++i) {
+        const float2 y = x[i];
+        m = make_float2(fmax_nn(m.x, y.x), fmax_nn(m.y, y.y));
+    }
+    return m;
+}
+
 typedef uint32_t un_u4 __attribute__((ext_vector_type(4), aligned(4)));
 typedef uint32_t un_u2 __attribute__((ext_vector_type(2), aligned(2)));
+template <typename MetaT>
+using MetaBits = std::conditional_t<sizeof(MetaT) == 2, uint16_t, uint32_t>;
 
-// One workgroup's share [t0, t1) of the prefix's tiles of one kind, for rows row0 .. of one KV head. DC: 32-channel
-// chunks of a head. RT: 16-row tiles per wave. WM x WT waves: WM share a tile and take other rows, WT take other tiles.
-template <int DC, int RT, int WM, int WT, bool PACKED>
+// Asks for an order of the block's instructions: a few vector ones behind each
+// of M matrix ones, whose pipe then runs while they issue. (Left alone the
+// compiler puts all matrix instructions first.)
+template <int M>
+__device__ __forceinline__ void interleave() {
+#pragma unroll
+    for (int i = 0; i < M; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+        __builtin_amdgcn_sched_group_barrier(0x002, 3, 0);  // VALU
+    }
+}
+
+typedef float mf_f16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ mf_f16 mfma32x32x16(const mf_u4 a, const mf_u4 b, const mf_f16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(mf_h8, a), __builtin_bit_cast(mf_h8, b), c, 0, 0, 0);
+}
+
+// For operands that are never NaN (fmaxf would quiet those it cannot see the origin of).
+__device__ __forceinline__ float max3(const float a, const float b, const float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+
+// Loads from a uniform base at a 32-bit lane offset in bytes. (The offset is opaque, or its 64-bit sum with the base
+// is formed in vector registers.)
+template <typename T>
+__device__ __forceinline__ T load_at(const void* base, uint32_t off) {
+    asm("" : "+v"(off));
+    return *reinterpret_cast<const T*>(static_cast<const char*>(base) + off);
+}
+
+// A loaded value that is used from here on: its uses (and the wait for it) do not move further up.
+template <typename T>
+__device__ __forceinline__ void pin(T& x) {
+    asm volatile("" : "+v"(x));
+}
+__device__ __forceinline__ void pin(mf_u4& x, const int e) {
+    uint32_t y = x[e];
+    asm volatile("" : "+v"(y));
+    x[e] = y;
+}
+
+// Ends a group of instructions that the scheduler may not mix with the next.
+__device__ __forceinline__ void slot_end() { __builtin_amdgcn_sched_barrier(0); }
+
+// One workgroup's share [t0, t1) of the prefix's tiles of one kind, for rows row0 .. of one KV head, head_dim up to
+// 32 DC. WM waves of 32 rows each, on the same tile.
+//
+//   QK  A = K (32 tokens x 16 channels), B = Q (16 channels x 32 rows): lane (h = lane / 32, n = lane % 32) receives
+//       tokens 8 (r / 4) + 4 h + r % 4 of row n, r < 16.
+//   PV  A = P (32 rows x 16 tokens), B = V (16 tokens x 32 channels): a lane's values r = 8 j .. 8 j + 7 are its A operand
+//       of step j, so V's tokens lie in LDS in the order position 16 j + 8 h + i <-> token 16 j + 8 (i / 4) + 4 h + i % 4.
+//
+// While the matrix cores multiply Q with K of tile k, the VALU stages tile
+// k + 1, whose loads went out a tile earlier. One barrier per tile. The order of
+// the two kinds of instructions is written out (a matrix instruction, then
+// vector ones while it runs): left alone the compiler puts all matrix
+// instructions first, each behind the wait for its LDS operands.
+template <int DC, int WM, bool PACKED, typename MetaT>
 __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, const Tiers& t, const int kvh,
                                             const int row0, const int rows, const int t0, const int t1,
                                             const int slot) {
-    using C = Config<DC, RT, WM, WT>;
     using L = TileLds<DC>;
-    constexpr int NK = (DC + WM - 1) / WM, NV = NK;  // K (V) units of a wave: 64 lanes x (4 tokens x 4 channels)
-    constexpr bool APART = WM >= 2 * DC;             // enough waves for K and V apart
+    constexpr bool F16M = sizeof(MetaT) == 2;
+    constexpr int ST = 2 * DC;  // QK steps
+    float neg1 = -1.0f;
+    asm("" : "+s"(neg1));
+    auto parts = [&](const float x0, const float x1) { return tt::parts(x0, x1, neg1); };
     const int lane = threadIdx.x & 63;
     const int wave = scalar(static_cast<int>(threadIdx.x) >> 6);
-    const int wm = wave % WM, wt = wave / WM;
-    const int n = lane & 15, g = lane >> 4;
+    const int n = lane & 31, h = lane >> 5;
     const int G = a.Hq / a.Hkv;
     const int D = a.D;
-    const size_t Hkv = static_cast<size_t>(a.Hkv);
-    // Waves that share a tile take its units in turn (DC: none): K's from the first wave on, V's from the wave behind
-    // them, or from the last wave backwards.
-    auto kunit = [&](const int i) { return wm + WM * i; };
-    auto vunit = [&](const int i) { return APART ? (wm >= DC ? wm - DC : DC) : WM - 1 - wm + WM * i; };
-
-    // K units: lane = (token quad, channel quad); V units the other way round,
-    // so that the writes of V's transposed rows spread over the banks.
+    const uint32_t stride = static_cast<uint32_t>(a.Hkv) * D;  // elements between tokens (blocks) of a head
+    // A unit is 64 lanes x (4 tokens x 4 channels) of a tile: 32 channels. Every wave stages the same share of a K and of
+    // a V unit: NT tokens and NC channels of each lane's. (With three units some waves repeat the last one's.)
+    constexpr int UNITS = DC == 3 ? 4 : DC, SHARES = WM / UNITS, NT = 4 / SHARES, NC = 4 / SHARES;
+    const int unit = min(wave % UNITS, DC - 1), part = wave / UNITS;
+    // K: lane = (token quad, channel quad); V the other way round, so that the
+    // writes of V's transposed rows spread over the banks.
     const int ktq = lane >> 3, kcq = lane & 7;
     const int vtq = lane & 7, vcq = lane >> 3;
-    const bool f16m = a.meta_fp16 != 0;
+    const int kc = 32 * unit + 4 * kcq, vc = 32 * unit + 4 * vcq;  // first channels
+    const int kt0 = 4 * ktq + NT * part;                           // first token
 
     // The tile in flight, as it lies in memory.
-    mf_u4 kx[NK][PACKED ? 3 : 4];  // packed: words, scale, zero; FP32: 4 tokens
-    mf_u4 vx[NV][PACKED ? 1 : 4];
+    mf_u4 kx[PACKED ? 3 : NT];        // packed: words, scale, zero; FP32: tokens
+    uint32_t vx[4][PACKED ? 1 : NC];  // packed: words of 4 tokens; FP32: 4 tokens' channels
     uint2 idv = make_uint2(0u, 0u);
-    uint32_t vm = 0u;              // packed: V scale (lanes 0-31) or zero (lanes 32-63) of token lane % 32
+    uint32_t vm = 0u;                 // packed: V scale (lanes 0-31) or zero (lanes 32-63) of token lane % 32
+    // The lane as a value of its own: what is computed from it inside the loop is not kept in registers over it.
+    auto lane_now = [&]() {
+        int x = lane;
+        asm volatile("" : "+v"(x));
+        return x;
+    };
     auto fetch = [&](const int tile) {
-        const int s0 = kTile * tile;
+        const int ln = lane_now();
+        const int s0 = kTile * tile, last = (PACKED ? t.slots : t.nd) - 1 - s0;  // tokens past the last repeat it (they are masked)
+        const uint32_t ck = min(32 * unit + 4 * (ln & 7), D - 4), cv = min(32 * unit + 4 * (ln >> 3), D - 4);
         if constexpr (PACKED) {
-            const int last = t.slots - 1;
-            const int sl = min(s0 + (lane & 31), last);
-            idv = *reinterpret_cast<const uint2*>(t.ids + sl);
-#pragma unroll
-            for (int i = 0; i < NK; ++i) {
-                const int u = kunit(i);
-                if (u >= DC) break;
-                const int c = min(32 * u + 4 * kcq, D - 4);
-                const int s = min(s0 + 4 * ktq, last);
-                const size_t km = static_cast<size_t>(a.kgs == 32 ? s >> 5 : s >> 4) * Hkv * D + c;
-                kx[i][0] = *reinterpret_cast<const un_u4*>(t.kp + static_cast<size_t>(s >> 4) * Hkv * D + c);
-                if (!f16m) {
-                    kx[i][1] = *reinterpret_cast<const un_u4*>(t.ks + 4 * km);
-                    kx[i][2] = *reinterpret_cast<const un_u4*>(t.kz + 4 * km);
-                } else {
-                    const un_u2 ps = *reinterpret_cast<const un_u2*>(t.ks + 2 * km);
-                    const un_u2 pz = *reinterpret_cast<const un_u2*>(t.kz + 2 * km);
-                    kx[i][1] = mf_u4{ps[0], ps[1], 0u, 0u};
-                    kx[i][2] = mf_u4{pz[0], pz[1], 0u, 0u};
-                }
+            constexpr uint32_t M = sizeof(MetaT);
+            const uint32_t kw = (min(4 * (ln >> 3), last) >> 4) * stride + ck, km = a.kgs == 32 ? ck : kw;
+            const size_t kb = static_cast<size_t>(a.kgs == 32 ? s0 >> 5 : s0 >> 4) * stride * M;
+            idv = load_at<uint2>(t.ids + s0, 8u * min(ln & 31, last));
+            kx[0] = load_at<un_u4>(t.kp + static_cast<size_t>(s0 >> 4) * stride, 4u * kw);
+            if constexpr (!F16M) {
+                kx[1] = load_at<un_u4>(t.ks + kb, M * km);
+                kx[2] = load_at<un_u4>(t.kz + kb, M * km);
+            } else {
+                const un_u2 ps = load_at<un_u2>(t.ks + kb, M * km), pz = load_at<un_u2>(t.kz + kb, M * km);
+                kx[1] = mf_u4{ps[0], ps[1], pz[0], pz[1]};
             }
-            const char* vmp = lane < 32 ? t.vs : t.vz;
-            if (vunit(0) != 0)
-                ;  // another wave's
-            else if (!f16m)
-                vm = *reinterpret_cast<const uint32_t*>(vmp + 4 * (sl * Hkv));
-            else
-                vm = *reinterpret_cast<const uint16_t*>(vmp + 2 * (sl * Hkv));
+            // V's scales in lanes 0-31, its zeros in lanes 32-63
+            const char* from = (ln < 32 ? t.vs : t.vz) + static_cast<size_t>(s0) * a.Hkv * M;
+            vm = *reinterpret_cast<const MetaBits<MetaT>*>(from + static_cast<uint32_t>(min(ln & 31, last)) * a.Hkv * M);
+            const uint32_t words = stride / 16;
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int u = vunit(i);
-                if (u >= DC) break;
-                const int c = min(32 * u + 4 * vcq, D - 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    vx[i][0][j] = t.vp[static_cast<size_t>(min(s0 + 4 * vtq + j, last)) * Hkv * (D / 16) + (c >> 4)];
-            }
+            for (int j = 0; j < 4; ++j)
+                vx[j][0] = load_at<uint32_t>(t.vp + static_cast<size_t>(s0) * words,
+                                             4u * (min(4 * (ln & 7) + j, last) * words + (cv >> 4)));
         } else {
 #pragma unroll
-            for (int i = 0; i < NK; ++i) {
-                const int u = kunit(i);
-                if (u >= DC) break;
-                const int c = min(32 * u + 4 * kcq, D - 4);
+            for (int j = 0; j < NT; ++j)
+                kx[j] = load_at<un_u4>(t.dk + static_cast<size_t>(s0) * stride,
+                                       4u * (min(4 * (ln >> 3) + NT * part + j, last) * stride + ck));
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    kx[i][j] = *reinterpret_cast<const un_u4*>(t.dk + min(s0 + 4 * ktq + j, t.nd - 1) * Hkv * D + c);
-            }
+            for (int j = 0; j < 4; ++j) {
+                const float* from = t.dv + static_cast<size_t>(s0) * stride;
+                const uint32_t off = 4u * (min(4 * (ln & 7) + j, last) * stride + cv + NC * part);
+                if constexpr (NC == 1) {
+                    vx[j][0] = load_at<uint32_t>(from, off);
+                } else {
+                    typedef uint32_t un_nc __attribute__((ext_vector_type(NC), aligned(4)));
+                    const un_nc y = load_at<un_nc>(from, off);
 #pragma unroll
-            for (int i = 0; i < NV; ++i) {
-                const int u = vunit(i);
-                if (u >= DC) break;
-                const int c = min(32 * u + 4 * vcq, D - 4);
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    vx[i][j] = *reinterpret_cast<const un_u4*>(t.dv + min(s0 + 4 * vtq + j, t.nd - 1) * Hkv * D + c);
+                    for (int e = 0; e < NC; ++e) vx[j][e] = y[e];
+                }
             }
         }
     };
-    // Bit j: token j of the fetched tile is attended.
+    // Bit j: token j of the tile is attended (packed: of the K tile in flight).
     auto mask_of = [&](const int tile) -> uint32_t {
         const int left = (PACKED ? t.slots : t.nd) - kTile * tile;
         const uint32_t in = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
@@ -242,130 +326,640 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
         return in;
     };
 
-    float* peak = reinterpret_cast<float*>(lds + C::TILES * L::BYTES);  // [buffer or wave][key, value]
+    float* peak = reinterpret_cast<float*>(lds + 2 * L::BYTES);  // [tile's parity][key, value]
     // A tile's largest key or value where it asks for another scale: too large for f16 at this one, or (first) any.
-    // The peaks only grow and so do the exponents after the first: none is ever cleared. Positive floats order like their bits. (An infinity has no scale that helps: it is left to make
-    // NaN of what reads it.)
+    // The peaks only grow and so do the exponents after the first: none is ever cleared. They are looked at once the
+    // tile's logits are there, which then are not used if they ask for another scale.
+    // Positive floats order like their bits. (An infinity has no scale that helps: it is left to make NaN of what
+    // reads it.)
     auto report = [&](const float x, const float back, const bool first, float* to) {
-        if (__ballot(x >= kLimit || (first && x > 0.0f)))
-            if ((x >= kLimit || (first && x > 0.0f)) && x < __builtin_huge_valf())
-                atomicMax(reinterpret_cast<int*>(to), __float_as_int(fminf(x * back, 3.0e38f)));
+        if ((x >= kLimit || (first && x > 0.0f)) && x < __builtin_huge_valf())
+            atomicMax(reinterpret_cast<int*>(to), __float_as_int(fminf(x * back, 3.0e38f)));
+    };
+
+    // Staging, in pieces to go between matrix instructions: f16 parts of the fetched K times 2^(4 - k_exp) ...
+    float ksc[4], kzr[4], kmx, vmx;
+    uint32_t kcodes, vcodes[2];
+    auto k_scale = [&](const int e, const uint32_t mask, const float by) {
+        // no attended token: the block's scale and zero may be anything
+        const bool any = ((mask >> (4 * ktq)) & 15u) != 0u && kc < D;
+        if constexpr (PACKED) {
+            pin(kx[1], F16M ? e >> 1 : e);
+            pin(kx[F16M ? 1 : 2], F16M ? 2 + (e >> 1) : e);
+            if constexpr (F16M) {
+                const uint32_t hs = kx[1][e >> 1], hz = kx[1][2 + (e >> 1)];
+                ksc[e] = (e & 1) ? half_hi(hs) : half_lo(hs);
+                kzr[e] = (e & 1) ? half_hi(hz) : half_lo(hz);
+            } else {
+                ksc[e] = __uint_as_float(kx[1][e]);
+                kzr[e] = __uint_as_float(kx[2][e]);
+            }
+            ksc[e] = any ? ksc[e] * by : 0.0f;
+            kzr[e] = any ? kzr[e] * by : 0.0f;
+            kmx = fmaxf(kmx, fmaxf(fabsf(kzr[e]), fabsf(__builtin_fmaf(3.0f, ksc[e], kzr[e]))));
+        }
+    };
+    auto k_gather = [&]() {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) pin(kx[0], e);
+        // the quad's codes, one byte per channel, from the lane's first token on
+        const uint32_t b = 0x0c0c0400u + 0x0101u * (ktq & 3);
+        const uint32_t lo = __builtin_amdgcn_perm(kx[0][1], kx[0][0], b);
+        const uint32_t hi = __builtin_amdgcn_perm(kx[0][3], kx[0][2], b);
+        kcodes = (lo | (hi << 16)) >> (2 * NT * part);
+    };
+    auto k_token = [&](char* tl, const int j, const uint32_t mask, const float by) {
+        float x[4];
+        if constexpr (PACKED) {
+            uint32_t y = (kcodes >> (2 * j)) & 0x03030303u;
+            asm("" : "+v"(y));  // (or every code is extracted by an instruction of its own)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(static_cast<float>((y >> (8 * e)) & 0xffu), ksc[e], kzr[e]);
+        } else {
+            const bool in = ((mask >> (kt0 + j)) & 1u) && kc < D;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) pin(kx[j], e);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[e] = in ? __uint_as_float(kx[j][e]) * by : 0.0f;
+                kmx = fmaxf(kmx, fabsf(x[e]));
+            }
+        }
+        const uint2 p = parts(x[0], x[1]), q = parts(x[2], x[3]);
+        char* d = tl + (kt0 + j) * L::KS + 2 * kc;
+        *reinterpret_cast<uint2*>(d + L::KHI) = make_uint2(p.x, q.x);
+        *reinterpret_cast<uint2*>(d + L::KLO) = make_uint2(p.y, q.y);
+    };
+    // ... and V: packed, the centred codes (2 q - 3) 4^(c % NC), exact, of channels c; FP32, f16 parts of V 2^(4 - v_exp).
+    // Token quad vtq in its place in the PV order.
+    const int vplace = 32 * (vtq >> 2) + 16 * (vtq & 1) + 8 * ((vtq >> 1) & 1);  // bytes
+    auto v_gather = [&]() {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) pin(vx[j][0]);
+        // the codes of the lane's first channel at bit 1 of each half
+        const uint32_t b = 0x0c040c00u + 0x00010001u * (vcq & 3);
+        vcodes[0] = (__builtin_amdgcn_perm(vx[1][0], vx[0][0], b) << 1) >> (2 * NC * part);
+        vcodes[1] = (__builtin_amdgcn_perm(vx[3][0], vx[2][0], b) << 1) >> (2 * NC * part);
+    };
+    auto v_channel = [&](char* tl, const int k, const uint32_t mask, const float by) {
+        char* d = tl + (vc + NC * part + k) * L::VS + vplace;
+        if constexpr (PACKED) {
+            // channels past head_dim hold codes of others, in columns that are not stored
+            const _Float16 c = static_cast<_Float16>(1024.0f + 3.0f * static_cast<float>(1 << (2 * k)));
+            const mf_h2 off = {c, c};
+            const uint32_t mk = 0x00060006u << (2 * k);
+            const mf_h2 z0 = __builtin_bit_cast(mf_h2, (vcodes[0] & mk) | 0x64006400u) - off;
+            const mf_h2 z1 = __builtin_bit_cast(mf_h2, (vcodes[1] & mk) | 0x64006400u) - off;
+            *reinterpret_cast<uint2*>(d + L::V) =
+                make_uint2(__builtin_bit_cast(uint32_t, z0), __builtin_bit_cast(uint32_t, z1));
+        } else {
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                pin(vx[j][k]);
+                y[j] = ((mask >> (4 * vtq + j)) & 1u) && vc < D ? __uint_as_float(vx[j][k]) * by : 0.0f;
+                vmx = fmaxf(vmx, fabsf(y[j]));
+            }
+            const uint2 p = parts(y[0], y[1]), q = parts(y[2], y[3]);
+            *reinterpret_cast<uint2*>(d + L::V) = make_uint2(p.x, q.x);
+            *reinterpret_cast<uint2*>(d + L::VLO) = make_uint2(p.y, q.y);
+        }
+    };
+    // Packed: V's scale 2^-v_exp and the zero of the centred codes, vz + 1.5 vs, of the tile's tokens, zeros where masked.
+    // (Every wave writes the same.)
+    auto stage_meta = [&](char* tl, const uint32_t mask, const int ve) {
+        pin(vm);
+        const float x = F16M ? half_lo(vm) : __uint_as_float(vm);
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        float y = lane < 32 ? x : __builtin_fmaf(1.5f, __uint_as_float(sw[0]), x);
+        y = ((mask >> n) & 1u) ? __builtin_amdgcn_ldexpf(y, -ve) : 0.0f;
+        reinterpret_cast<float*>(tl + L::VMETA)[lane] = y;
+        // a scale up to 2 2^v_exp stays in reach (P <= 2^14): in units of kLimit / 2
+        vmx = lane < 32 ? fabsf(y) * (0.5f * kLimit) : 0.0f;
+    };
+
+    fetch(t0);  // its loads go out before the queries'
+    float2 top;  // the first tile's largest key and value
+    {
+        const uint32_t m = mask_of(t0);
+        kmx = vmx = 0.0f;
+        if constexpr (PACKED) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) k_scale(e, m, 1.0f);
+            vmx = lane < 32 && ((m >> n) & 1u) ? fabsf(F16M ? half_lo(vm) : __uint_as_float(vm)) : 0.0f;
+        } else {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    kmx = fmaxf(kmx, ((m >> (kt0 + j)) & 1u) && kc < D ? fabsf(__uint_as_float(kx[j][e])) : 0.0f);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < NC; ++e)
+                    vmx = fmaxf(vmx, ((m >> (4 * vtq + j)) & 1u) && vc < D ? fabsf(__uint_as_float(vx[j][e])) : 0.0f);
+        }
+        top = group_max<WM>(kmx, vmx, lds, wave, lane);
+    }
+    // Q' = Q 2^(12 - e), e the exponent of the row's largest value: row n, channels 16 s + 8 h .. + 7.
+    const int rn = row0 + 32 * wave + n;
+    const bool live = rn < rows;
+    const int seq = live ? rn / G : 0;
+    const int head = kvh * G + (live ? rn % G : 0);
+    mf_u4 qh[ST], ql[ST];
+    float crow;  // log2 units per unit of the product
+    {
+        const float* q = global_ptr(a.seqs[seq].Q) + static_cast<size_t>(head) * D;
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+            const int c = min(16 * s + 8 * h, D - 8);
+            qh[s] = *reinterpret_cast<const un_u4*>(q + c);
+            ql[s] = *reinterpret_cast<const un_u4*>(q + c + 4);
+        }
+#pragma unroll
+        for (int s = 0; s < ST; ++s)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if (!live || 16 * s + 8 * h >= D) qh[s][j] = ql[s][j] = 0u;
+                mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(qh[s][j])), fabsf(__uint_as_float(ql[s][j]))));
+            }
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        const int e = (mx > 0.0f) ? __builtin_amdgcn_frexp_expf(mx) : 0;
+#pragma unroll
+        for (int s = 0; s < ST; ++s) {
+            uint2 p[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const mf_u4 x = j < 2 ? qh[s] : ql[s];
+                p[j] = parts(__builtin_amdgcn_ldexpf(__uint_as_float(x[2 * (j & 1)]), 12 - e),
+                             __builtin_amdgcn_ldexpf(__uint_as_float(x[2 * (j & 1) + 1]), 12 - e));
+            }
+            qh[s] = mf_u4{p[0].x, p[1].x, p[2].x, p[3].x};
+            ql[s] = mf_u4{p[0].y, p[1].y, p[2].y, p[3].y};
+        }
+        crow = __builtin_amdgcn_ldexpf(a.scale2, e - 16);
+    }
+
+    mf_f16 acc[DC];
+    float mr = -3.0e38f, l = 0.0f, pz = 0.0f;
+#pragma unroll
+    for (int s = 0; s < DC; ++s)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[s][r] = 0.0f;
+    // Exponents of the scales of K and V (uniform over the workgroup), and whether no tile has set them yet.
+    int k_exp = exponent(top.x, 8), v_exp = exponent(top.y, PACKED ? 0 : 8);
+    bool kfirst = !__ballot(top.x > 0.0f), vfirst = !__ballot(top.y > 0.0f);
+    if (threadIdx.x < 4) peak[threadIdx.x] = 0.0f;
+
+    // At the top of the loop tile k is staged and tile k + 1 in flight. `again`: tile k is in flight and has to be staged,
+    // at the start or with other exponents; its products are not used then.
+    int again = 1;
+    asm("" : "+s"(again));  // (or the compiler makes a loop of its own of the start)
+    uint32_t mask = 0u;  // of tile k
+    int k = t0;
+#pragma unroll 1
+    do {
+        lds_barrier();
+        const float pk_k = peak[2 * (k & 1)], pk_v = peak[2 * (k & 1) + 1];
+        const int next = min(again ? k : k + 1, t1 - 1);  // the tile in flight
+        const char* tl = lds + (k & 1) * L::BYTES;
+        uint32_t mnext = 0u;
+        mf_f16 d;
+        {
+            // QK of tile k, between its instructions the tile in flight to LDS.
+            const char* kl = tl + n * L::KS + 16 * h;
+            const int to = again ? k & 1 : (k + 1) & 1;
+            char* dst = lds + to * L::BYTES;
+            const float kby = __builtin_amdgcn_ldexpf(16.0f, -k_exp), vby = __builtin_amdgcn_ldexpf(16.0f, -v_exp);
+            constexpr int PIECES = PACKED ? 8 + NT + NC : 1 + NT + NC, SLOTS = 3 * ST;
+            auto piece = [&](const int i) {
+                if (i == 0) {
+                    pin(idv.x);
+                    pin(idv.y);
+                    mnext = mask_of(next);
+                    kmx = vmx = 0.0f;
+                } else if (PACKED && i < 5) {
+                    k_scale(i - 1, mnext, kby);
+                } else if (PACKED && i == 5) {
+                    k_gather();
+                } else if (i < (PACKED ? 6 : 1) + NT) {
+                    k_token(dst, i - (PACKED ? 6 : 1), mnext, kby);
+                } else if (PACKED && i == 6 + NT) {
+                    v_gather();
+                } else if (PACKED && i == 7 + NT) {
+                    stage_meta(dst, mnext, v_exp);
+                } else {
+                    v_channel(dst, i - (PACKED ? 8 : 1) - NT, mnext, vby);
+                }
+            };
+            mf_u4 kh[2], kw[2];
+            auto load_k = [&](const int s) {
+                kh[s & 1] = *reinterpret_cast<const mf_u4*>(kl + L::KHI + 32 * s);
+                kw[s & 1] = *reinterpret_cast<const mf_u4*>(kl + L::KLO + 32 * s);
+            };
+            load_k(0);
+            slot_end();
+#pragma unroll
+            for (int r = 0; r < 16; ++r) d[r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i) {
+                const int s = i / 3;
+                if (i % 3 == 0 && s + 1 < ST) load_k(s + 1);
+                d = mfma32x32x16(i % 3 == 2 ? kw[s & 1] : kh[s & 1], i % 3 == 0 ? ql[s] : qh[s], d);
+#pragma unroll
+                for (int o = i * PIECES / SLOTS; o < (i + 1) * PIECES / SLOTS; ++o) piece(o);
+                slot_end();
+            }
+            if (__ballot(fmaxf(kmx, vmx) >= kLimit) || kfirst || vfirst) {
+                report(kmx, __builtin_amdgcn_ldexpf(0.0625f, k_exp), kfirst, peak + 2 * to);
+                report(vmx, __builtin_amdgcn_ldexpf(PACKED ? 2.0f / kLimit : 0.0625f, v_exp), vfirst, peak + 2 * to + 1);
+            }
+        }
+        int ahead = again ? k + 1 : k + 2;  // the tile to fetch
+        const int skip = again;
+        if (!again && __ballot(fmaxf(pk_k, pk_v) > 0.0f)) {
+            int kn = k_exp, vn = v_exp;
+            if (__ballot(pk_k > 0.0f)) {
+                const int e = exponent(pk_k, 8);  // (a peak past the limit asks for at least k_exp + 1 at 11)
+                if (e - 3 > k_exp || kfirst) kn = e;
+                kfirst = false;
+            }
+            if (__ballot(pk_v > 0.0f)) {
+                const int e = exponent(pk_v, PACKED ? 0 : 8);
+                if (e - (PACKED ? 1 : 3) > v_exp || vfirst) vn = e;
+                vfirst = false;
+            }
+            if (kn != k_exp || vn != v_exp) {
+                const float f = __builtin_amdgcn_ldexpf(1.0f, v_exp - vn);
+                pz *= f;
+#pragma unroll
+                for (int s = 0; s < DC; ++s) acc[s] *= f;
+                k_exp = kn;
+                v_exp = vn;
+                again = 2;
+                ahead = k;
+            }
+        }
+        // (The one place in the loop that fetches: of several, copies would be made, which wait for the loads.)
+        fetch(min(ahead, t1 - 1));
+        again = again == 2 ? 1 : 0;
+        if (!(skip | again)) {
+            mf_u4 vh[2], vw[2];
+            auto load_v = [&](const int s) {  // step s: channels 32 (s / 2) .., tokens of half s % 2
+                const char* x = tl + (32 * (s >> 1) + n) * L::VS + 32 * (s & 1) + 16 * h;
+                vh[s & 1] = *reinterpret_cast<const mf_u4*>(x + L::V);
+                if constexpr (!PACKED) vw[s & 1] = *reinterpret_cast<const mf_u4*>(x + L::VLO);
+            };
+            // Softmax: P (packed: P times V's scale) as the PV A operand.
+            if (mask != 0xffffffffu) {
+                const uint32_t mine = mask >> (4 * (lane_now() >> 5));
+#pragma unroll
+                for (int r = 0; r < 16; ++r) d[r] = ((mine >> (8 * (r >> 2) + (r & 3))) & 1u) ? d[r] : kNegInf;
+            }
+            const float c = __builtin_amdgcn_ldexpf(crow, k_exp);
+            float mx = max3(max3(d[0], d[1], d[2]), max3(d[3], d[4], d[5]), max3(d[6], d[7], d[8]));
+            mx = max3(mx, max3(d[9], d[10], d[11]), max3(d[12], d[13], max3(d[14], d[15], d[15])));
+            mx = __builtin_fmaf(mx, c, -kUp);
+            // the reference moves only when a row's maximum passes it by more than the slack
+            if (__ballot(mx > mr + kSlack)) {
+                const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+                mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+                const bool up = mx > mr + kSlack;
+                const float mn = up ? mx : mr;
+                const float al = up ? __builtin_amdgcn_exp2f(mr - mn) : 1.0f;
+                l *= al;
+                pz *= al;
+                const int from = 16 * (lane_now() >> 5);  // bytes: the lane group's first row
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const float ar = __int_as_float(__builtin_amdgcn_ds_bpermute(from + 4 * (8 * (r >> 2) + (r & 3)), __float_as_int(al)));
+#pragma unroll
+                    for (int s = 0; s < DC; ++s) acc[s][r] *= ar;
+                }
+                mr = mn;
+            }
+            mf_u4 ph[2], pl[2];
+            load_v(0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                mf_f4 vs, vz;
+                if constexpr (PACKED) {
+                    vs = *reinterpret_cast<const mf_f4*>(tl + L::VMETA + 32 * j + 16 * h);
+                    vz = *reinterpret_cast<const mf_f4*>(tl + L::VMETA + 128 + 32 * j + 16 * h);
+                }
+                float p[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(d[4 * j + r], c, -mr));
+                l += (p[0] + p[1]) + (p[2] + p[3]);
+                if constexpr (PACKED) {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        pz = __builtin_fmaf(p[r], vz[r], pz);
+                        p[r] *= vs[r];
+                    }
+                }
+#pragma unroll
+                for (int x = 0; x < 2; ++x) {
+                    const uint2 y = parts(p[2 * x], p[2 * x + 1]);
+                    ph[j >> 1][2 * (j & 1) + x] = y.x;
+                    pl[j >> 1][2 * (j & 1) + x] = y.y;
+                }
+            }
+            constexpr int PR = PACKED ? 2 : 3, SLOTS = 2 * DC * PR;
+            slot_end();
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i) {
+                const int s = i / PR, q = i % PR;
+                if (q == 0 && s + 1 < 2 * DC) load_v(s + 1);
+                acc[s >> 1] = mfma32x32x16(q == 0 ? pl[s & 1] : ph[s & 1], !PACKED && q == 1 ? vw[s & 1] : vh[s & 1], acc[s >> 1]);
+                slot_end();
+            }
+        }
+        mask = mnext;
+        k += skip | again ? 0 : 1;
+    } while (k < t1);
+
+    // The partial in units of V: acc holds 16 V 2^-v_exp (FP32 tiles), or 2 4^(c % NC) of it without the centred zero.
+    auto both = [&](const float x) {  // a row's sum over its two lanes
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    };
+    l = both(l);
+    const float z = PACKED ? __builtin_amdgcn_ldexpf(both(pz), v_exp) : 0.0f;
+    const float back = __builtin_amdgcn_ldexpf(1.0f, v_exp - (PACKED ? 1 + 2 * (n & (NC - 1)) : 4));
+    // row n's partial, behind its sequence's own slots
+    const int ns = a.slot_base[seq + 1] - a.slot_base[seq];
+    const uint32_t pi = static_cast<uint32_t>(a.slot_base[seq] * a.Hq + head * ns + (ns - a.prefix_slots + slot));
+    if (h == 0 && live) {
+        a.ml[2 * static_cast<size_t>(pi)] = l > 0.0f ? mr : kNegInf;
+        a.ml[2 * static_cast<size_t>(pi) + 1] = l;
+    }
+    const int first = 4 * (lane_now() >> 5);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int row = 8 * (r >> 2) + first + (r & 3);
+        const float zr = PACKED ? __shfl(z, row, 64) : 0.0f;
+        const uint32_t pr = static_cast<uint32_t>(__shfl(static_cast<int>(pi), row, 64));
+        if (row0 + 32 * wave + row >= rows) continue;
+        float* o = a.acc + static_cast<size_t>(pr) * D + n;
+#pragma unroll
+        for (int s = 0; s < DC; ++s)
+            if (32 * s + n < D) o[32 * s] = __builtin_fmaf(acc[s][r], back, zr);
+    }
+}
+
+// The same for head dims above 128, whose accumulators leave registers for 16 rows per wave. DC: 32-channel
+// chunks of a head. RT: 16-row tiles per wave. WM: waves, on the same tile with rows of their own.
+//
+// The loop is a pipeline over the tiles: while the matrix cores multiply Q with
+// K of tile k, the VALU turns tile k - 1's logits into P; while they multiply P
+// with V of tile k - 1, it stages K of tile k + 1 and V of tile k, whose loads
+// went out at the top. One barrier per tile.
+template <int DC, int RT, int WM, bool PACKED, typename MetaT>
+__device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const Tiers& t, const int kvh,
+                                            const int row0, const int rows, const int t0, const int t1,
+                                            const int slot) {
+    using L = TileLds<DC>;
+    static_assert(WM >= DC || WM >= 4, "a K and a V unit per wave at most");
+    constexpr bool F16M = sizeof(MetaT) == 2;
+    float neg1 = -1.0f;
+    asm("" : "+s"(neg1));
+    auto parts = [&](const float x0, const float x1) { return tt::parts(x0, x1, neg1); };
+    const int lane = threadIdx.x & 63;
+    const int wave = scalar(static_cast<int>(threadIdx.x) >> 6);
+    const int n = lane & 15, g = lane >> 4;
+    const int G = a.Hq / a.Hkv;
+    const int D = a.D;
+    const size_t Hkv = static_cast<size_t>(a.Hkv);
+    // A unit is 64 lanes x (4 tokens x 4 channels) of a tile: 32 channels. Where the waves are a multiple of the units,
+    // every wave has a K and a V unit's share (NT tokens, or NC channels, of each lane's); else the first waves stage
+    // K's and, with enough waves, the ones behind them V's, or the last waves backwards.
+    constexpr bool EVEN = WM % DC == 0, APART = !EVEN && WM >= 2 * DC;
+    constexpr int SHARES = EVEN ? WM / DC : 1, NT = 4 / SHARES, NC = 4 / SHARES;
+    const int ku = EVEN ? wave % DC : wave, vu = EVEN ? ku : (APART ? wave - DC : WM - 1 - wave);
+    const int part = EVEN ? wave / DC : 0;
+    const bool has_k = EVEN || ku < DC, has_v = EVEN || (vu >= 0 && vu < DC);
+    // K units: lane = (token quad, channel quad); V units the other way round,
+    // so that the writes of V's transposed rows spread over the banks.
+    const int ktq = lane >> 3, kcq = lane & 7;
+    const int vtq = lane & 7, vcq = lane >> 3;
+    const int kc = 32 * ku + 4 * kcq, vc = 32 * vu + 4 * vcq;  // first channels
+    const int kt0 = 4 * ktq + NT * part;                       // first token
+    const bool has_meta = vu == 0 && part == 0;                // stages V's scales and zeros
+
+    // The tile in flight, as it lies in memory.
+    mf_u4 kx[PACKED ? 3 : NT];               // packed: words, scale, zero; FP32: tokens
+    uint32_t vx[4][PACKED ? 1 : NC];         // packed: words of 4 tokens; FP32: 4 tokens' channels
+    uint2 idv = make_uint2(0u, 0u);
+    uint32_t vm = 0u;                        // packed: V scale (lanes 0-31) or zero (lanes 32-63) of token lane % 32
+    auto fetch_k = [&](const int tile) {
+        const int s0 = kTile * tile;
+        const int c = min(kc, D - 4);
+        if constexpr (PACKED) {
+            const int last = t.slots - 1;
+            idv = *reinterpret_cast<const uint2*>(t.ids + min(s0 + (lane & 31), last));
+            if (has_k) {
+                const int s = min(s0 + 4 * ktq, last);
+                const size_t km = static_cast<size_t>(a.kgs == 32 ? s >> 5 : s >> 4) * Hkv * D + c;
+                kx[0] = *reinterpret_cast<const un_u4*>(t.kp + static_cast<size_t>(s >> 4) * Hkv * D + c);
+                if constexpr (!F16M) {
+                    kx[1] = *reinterpret_cast<const un_u4*>(t.ks + 4 * km);
+                    kx[2] = *reinterpret_cast<const un_u4*>(t.kz + 4 * km);
+                } else {
+                    const un_u2 ps = *reinterpret_cast<const un_u2*>(t.ks + 2 * km);
+                    const un_u2 pz = *reinterpret_cast<const un_u2*>(t.kz + 2 * km);
+                    kx[1] = mf_u4{ps[0], ps[1], pz[0], pz[1]};
+                }
+            }
+        } else if (has_k) {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+                kx[j] = *reinterpret_cast<const un_u4*>(t.dk + min(s0 + kt0 + j, t.nd - 1) * Hkv * D + c);
+        }
+    };
+    auto fetch_v = [&](const int tile) {
+        if (!has_v) return;
+        const int s0 = kTile * tile;
+        const int c = min(vc, D - 4);
+        if constexpr (PACKED) {
+            const int last = t.slots - 1;
+            if (has_meta) {
+                const size_t at = min(s0 + (lane & 31), last) * Hkv * sizeof(MetaT);
+                vm = *reinterpret_cast<const MetaBits<MetaT>*>((lane < 32 ? t.vs : t.vz) + at);
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                vx[j][0] = t.vp[static_cast<size_t>(min(s0 + 4 * vtq + j, last)) * Hkv * (D / 16) + (c >> 4)];
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                typedef uint32_t un_nc __attribute__((ext_vector_type(NC), aligned(4)));
+                const float* x = t.dv + min(s0 + 4 * vtq + j, t.nd - 1) * Hkv * D + c + NC * part;
+                if constexpr (NC == 1) {
+                    vx[j][0] = __float_as_uint(*x);
+                } else {
+                    const un_nc y = *reinterpret_cast<const un_nc*>(x);
+#pragma unroll
+                    for (int e = 0; e < NC; ++e) vx[j][e] = y[e];
+                }
+            }
+        }
+    };
+    // Bit j: token j of the tile is attended (packed: of the K tile in flight).
+    auto mask_of = [&](const int tile) -> uint32_t {
+        const int left = (PACKED ? t.slots : t.nd) - kTile * tile;
+        const uint32_t in = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+        if constexpr (PACKED) return static_cast<uint32_t>(__ballot((idv.x & idv.y) != 0xffffffffu)) & in;
+        return in;
+    };
+
+    float* peak = reinterpret_cast<float*>(lds + 2 * L::BYTES);  // [tile's parity][key, value]
+    // A tile's largest key or value where it asks for another scale: too large for f16 at this one, or (first) any.
+    // The peaks only grow and so do the exponents after the first: none is ever cleared.
+    // Positive floats order like their bits. (An infinity has no scale that helps: it is left to make NaN of what
+    // reads it.)
+    auto report = [&](const float x, const float back, const bool first, float* to) {
+        const bool tell = x >= kLimit || (first && x > 0.0f);
+        if (__ballot(tell))
+            if (tell && x < __builtin_huge_valf()) atomicMax(reinterpret_cast<int*>(to), __float_as_int(fminf(x * back, 3.0e38f)));
     };
 
     // f16 parts of the fetched K (scaled by 2^(4 - ke)).
-    auto stage_k = [&](char* tl, const uint32_t mask, const int ke, const bool first, float* to) {
+    auto stage_k = [&](char* tl, const uint32_t mask, const int ke) -> float {
         const float ksc = __builtin_amdgcn_ldexpf(16.0f, -ke);
-        const uint32_t mine = (mask >> (4 * ktq)) & 15u;
         float mx = 0.0f;
+        float x[NT][4];  // [token][channel]
+        if constexpr (PACKED) {
+            // no attended token: the block's scale and zero may be anything
+            const bool any = ((mask >> (4 * ktq)) & 15u) != 0u && kc < D;
+            float sc[4], zr[4];
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-            const int u = kunit(i);
-            if (u >= DC) break;
-            const int c0 = 32 * u + 4 * kcq;
-            float x[4][4];  // [token][channel]
-            if constexpr (PACKED) {
-                // no attended token: the block's scale and zero may be anything
-                const bool any = mine != 0u && c0 < D;
-                float sc[4], zr[4];
+            for (int e = 0; e < 4; ++e) {
+                if constexpr (F16M) {
+                    const uint32_t hs = kx[1][e >> 1], hz = kx[1][2 + (e >> 1)];
+                    sc[e] = (e & 1) ? half_hi(hs) : half_lo(hs);
+                    zr[e] = (e & 1) ? half_hi(hz) : half_lo(hz);
+                } else {
+                    sc[e] = __uint_as_float(kx[1][e]);
+                    zr[e] = __uint_as_float(kx[2][e]);
+                }
+                sc[e] = any ? sc[e] * ksc : 0.0f;
+                zr[e] = any ? zr[e] * ksc : 0.0f;
+                mx = fmaxf(mx, fmaxf(fabsf(zr[e]), fabsf(__builtin_fmaf(3.0f, sc[e], zr[e]))));
+            }
+            // the quad's codes, one byte per channel, then one code per byte
+            const uint32_t b = 0x0c0c0400u + 0x0101u * (ktq & 3);
+            const uint32_t lo = __builtin_amdgcn_perm(kx[0][1], kx[0][0], b);
+            const uint32_t hi = __builtin_amdgcn_perm(kx[0][3], kx[0][2], b);
+            const uint32_t w = (lo | (hi << 16)) >> (2 * NT * part);
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                uint32_t y = (w >> (2 * j)) & 0x03030303u;
+                asm("" : "+v"(y));  // (or every code is extracted by an instruction of its own)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    x[j][e] = __builtin_fmaf(static_cast<float>((y >> (8 * e)) & 0xffu), sc[e], zr[e]);
+            }
+        } else {
+            const uint32_t mine = mask >> kt0;
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    const uint32_t ws = kx[i][1][e], wz = kx[i][2][e];
-                    const uint32_t hs = kx[i][1][e >> 1], hz = kx[i][2][e >> 1];
-                    const float s = f16m ? ((e & 1) ? half_hi(hs) : half_lo(hs)) : __uint_as_float(ws);
-                    const float z = f16m ? ((e & 1) ? half_hi(hz) : half_lo(hz)) : __uint_as_float(wz);
-                    sc[e] = any ? s * ksc : 0.0f;
-                    zr[e] = any ? z * ksc : 0.0f;
-                    mx = fmax_abs_nn(mx, fmax_abs_nn(zr[e], __builtin_fmaf(3.0f, sc[e], zr[e])));
+                    x[j][e] = ((mine >> j) & 1u) && kc < D ? __uint_as_float(kx[j][e]) * ksc : 0.0f;
+                    mx = fmaxf(mx, fabsf(x[j][e]));
                 }
-                // the quad's codes, one byte per channel, then one code per byte
-                const uint32_t b = 0x0c0c0400u + 0x0101u * (ktq & 3);
-                const uint32_t lo = __builtin_amdgcn_perm(kx[i][0][1], kx[i][0][0], b);
-                const uint32_t hi = __builtin_amdgcn_perm(kx[i][0][3], kx[i][0][2], b);
-                const uint32_t w = lo | (hi << 16);
+        }
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            const uint2 p = parts(x[j][0], x[j][1]), q = parts(x[j][2], x[j][3]);
+            char* d = tl + (kt0 + j) * L::KS + 2 * kc;
+            *reinterpret_cast<uint2*>(d + L::KHI) = make_uint2(p.x, q.x);
+            *reinterpret_cast<uint2*>(d + L::KLO) = make_uint2(p.y, q.y);
+        }
+        return mx;
+    };
+    // Packed: the centred codes (2 q - 3) 4^(c % NC), exact, of channels c. FP32: f16 parts of V 2^(4 - ve). Token quad vtq
+    // sits in the MFMA order: 8 tokens per lane group, its half by the 16-token tile.
+    auto stage_v = [&](char* tl, const uint32_t mask, const int ve) -> float {
+        float mx = 0.0f;
+        char* d = tl + (vc + NC * part) * L::VS + 16 * (vtq & 3) + 8 * (vtq >> 2);
+        if constexpr (PACKED) {
+            // channels past head_dim hold codes of others, in columns that are not stored
+            const uint32_t b = 0x0c040c00u + 0x00010001u * (vcq & 3);
+            // the codes of the lane's first channel at bit 1 of each half
+            const uint32_t y0 = (__builtin_amdgcn_perm(vx[1][0], vx[0][0], b) << 1) >> (2 * NC * part);
+            const uint32_t y1 = (__builtin_amdgcn_perm(vx[3][0], vx[2][0], b) << 1) >> (2 * NC * part);
+#pragma unroll
+            for (int k = 0; k < NC; ++k) {
+                const _Float16 c = static_cast<_Float16>(1024.0f + 3.0f * static_cast<float>(1 << (2 * k)));
+                const mf_h2 off = {c, c};
+                const uint32_t mk = 0x00060006u << (2 * k);
+                const mf_h2 z0 = __builtin_bit_cast(mf_h2, (y0 & mk) | 0x64006400u) - off;
+                const mf_h2 z1 = __builtin_bit_cast(mf_h2, (y1 & mk) | 0x64006400u) - off;
+                *reinterpret_cast<uint2*>(d + k * L::VS + L::V) =
+                    make_uint2(__builtin_bit_cast(uint32_t, z0), __builtin_bit_cast(uint32_t, z1));
+            }
+        } else {
+            const float vsc = __builtin_amdgcn_ldexpf(16.0f, -ve);
+            const uint32_t mine = (mask >> (4 * vtq)) & 15u;
+#pragma unroll
+            for (int e = 0; e < NC; ++e) {
+                float y[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    uint32_t y = (w >> (2 * j)) & 0x03030303u;
-                    asm("" : "+v"(y));  // (or every code is extracted by an instruction of its own)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        x[j][e] = __builtin_fmaf(static_cast<float>((y >> (8 * e)) & 0xffu), sc[e], zr[e]);
+                    y[j] = ((mine >> j) & 1u) && vc < D ? __uint_as_float(vx[j][e]) * vsc : 0.0f;
+                    mx = fmaxf(mx, fabsf(y[j]));
                 }
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        x[j][e] = ((mine >> j) & 1u) && c0 < D ? __uint_as_float(kx[i][j][e]) * ksc : 0.0f;
-                        mx = fmaxf(mx, fabsf(x[j][e]));
-                    }
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint2 p = parts(x[j][0], x[j][1]), q = parts(x[j][2], x[j][3]);
-                char* d = tl + (4 * ktq + j) * L::KS + 2 * c0;
-                *reinterpret_cast<uint2*>(d + L::KHI) = make_uint2(p.x, q.x);
-                *reinterpret_cast<uint2*>(d + L::KLO) = make_uint2(p.y, q.y);
+                const uint2 p = parts(y[0], y[1]), q = parts(y[2], y[3]);
+                *reinterpret_cast<uint2*>(d + e * L::VS + L::V) = make_uint2(p.x, q.x);
+                *reinterpret_cast<uint2*>(d + e * L::VS + L::VLO) = make_uint2(p.y, q.y);
             }
         }
-        report(mx, __builtin_amdgcn_ldexpf(0.0625f, ke), first, to);
+        return mx;
     };
-    // Packed: the centred codes (2 q - 3) 4^(c % 4), exact, of channels c; FP32: f16 parts of V 2^(4 - ve). Token quad
-    // vtq sits in the MFMA order: 8 tokens per lane group, its half by the 16-token tile.
-    auto stage_v = [&](char* tl, const uint32_t mask, const int ve, const bool first, float* to) {
-        const float vsc = __builtin_amdgcn_ldexpf(16.0f, -ve);
-        const uint32_t mine = (mask >> (4 * vtq)) & 15u;
-        float mx = 0.0f;
-#pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            const int u = vunit(i);
-            if (u >= DC) break;
-            const int c0 = 32 * u + 4 * vcq;
-            char* d = tl + c0 * L::VS + 16 * (vtq & 3) + 8 * (vtq >> 2);
-            if constexpr (PACKED) {
-                // channels past head_dim hold codes of others, in columns that are not stored
-                const uint32_t b = 0x0c040c00u + 0x00010001u * (vcq & 3);
-                const uint32_t y0 = __builtin_amdgcn_perm(vx[i][0][1], vx[i][0][0], b) << 1;
-                const uint32_t y1 = __builtin_amdgcn_perm(vx[i][0][3], vx[i][0][2], b) << 1;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    const _Float16 c = static_cast<_Float16>(1024.0f + 3.0f * static_cast<float>(1 << (2 * k)));
-                    const mf_h2 off = {c, c};
-                    const uint32_t mk = 0x00060006u << (2 * k);
-                    const mf_h2 z0 = __builtin_bit_cast(mf_h2, (y0 & mk) | 0x64006400u) - off;
-                    const mf_h2 z1 = __builtin_bit_cast(mf_h2, (y1 & mk) | 0x64006400u) - off;
-                    *reinterpret_cast<uint2*>(d + k * L::VS + L::V) =
-                        make_uint2(__builtin_bit_cast(uint32_t, z0), __builtin_bit_cast(uint32_t, z1));
-                }
-            } else {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    float y[4];
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        y[j] = ((mine >> j) & 1u) && c0 < D ? __uint_as_float(vx[i][j][e]) * vsc : 0.0f;
-                        mx = fmaxf(mx, fabsf(y[j]));
-                    }
-                    const uint2 p = parts(y[0], y[1]), q = parts(y[2], y[3]);
-                    *reinterpret_cast<uint2*>(d + e * L::VS + L::V) = make_uint2(p.x, q.x);
-                    *reinterpret_cast<uint2*>(d + e * L::VS + L::VLO) = make_uint2(p.y, q.y);
-                }
-            }
-        }
-        if constexpr (!PACKED) report(mx, __builtin_amdgcn_ldexpf(0.0625f, ve), first, to);
-    };
-    // Packed: V's scale 2^-ve and the zero of the centred codes, vz + 1.5 vs, of the tile's tokens (zeros where masked).
-    auto stage_vmeta = [&](char* tl, const uint32_t mask, const int ve, const bool first, float* to) {
-        const float x = f16m ? half_lo(vm) : __uint_as_float(vm);
+    // Packed: V's scale 2^-ve and the zero of the centred codes, vz + 1.5 vs, of the tile's tokens, zeros where masked.
+    auto stage_meta = [&](char* tl, const uint32_t mask, const int ve) -> float {
+        const float x = F16M ? half_lo(vm) : __uint_as_float(vm);
         const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
         float y = lane < 32 ? x : __builtin_fmaf(1.5f, __uint_as_float(sw[0]), x);
         y = ((mask >> (lane & 31)) & 1u) ? __builtin_amdgcn_ldexpf(y, -ve) : 0.0f;
         reinterpret_cast<float*>(tl + L::VMETA)[lane] = y;
-        // a scale up to 2 2^ve stays in reach (P <= 2^14); reported in units of kLimit / 2
-        report(lane < 32 ? fabsf(y) * (0.5f * kLimit) : 0.0f, __builtin_amdgcn_ldexpf(2.0f / kLimit, ve), first, to);
+        return lane < 32 ? fabsf(y) : 0.0f;
     };
 
-    // The first tile's loads go out before the queries'.
-    if (t0 + wt < t1) fetch(t0 + wt);
+    fetch_k(t0);
+    fetch_v(t0);
+    float2 top;  // the first tile's largest key and value
+    {
+        const uint32_t m = mask_of(t0);
+        float kmx = 0.0f, vmx = 0.0f;
+        if constexpr (PACKED) {
+            const bool any = ((m >> (4 * ktq)) & 15u) != 0u && kc < D;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t hs = kx[1][F16M ? e >> 1 : e], hz = kx[F16M ? 1 : 2][F16M ? 2 + (e >> 1) : e];
+                const float sc = F16M ? ((e & 1) ? half_hi(hs) : half_lo(hs)) : __uint_as_float(hs);
+                const float zr = F16M ? ((e & 1) ? half_hi(hz) : half_lo(hz)) : __uint_as_float(hz);
+                if (any) kmx = fmaxf(kmx, fmaxf(fabsf(zr), fabsf(__builtin_fmaf(3.0f, sc, zr))));
+            }
+            if (has_meta && lane < 32 && ((m >> lane) & 1u)) vmx = fabsf(F16M ? half_lo(vm) : __uint_as_float(vm));
+        } else {
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (((m >> (kt0 + j)) & 1u) && kc < D) kmx = fmaxf(kmx, fabsf(__uint_as_float(kx[j][e])));
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int e = 0; e < NC; ++e)
+                    if (((m >> (4 * vtq + j)) & 1u) && vc < D) vmx = fmaxf(vmx, fabsf(__uint_as_float(vx[j][e])));
+        }
+        top = group_max<WM>(kmx, vmx, lds, wave, lane);
+    }
 
     // Q' = Q 2^(12 - e), e the exponent of the row's largest value, as the QK B operand: row n of row tile rt, channels
     // 32 s + 8 g .. + 7.
@@ -373,27 +967,26 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
     float crow[RT];  // log2 units per unit of the product
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-        const int r = row0 + 16 * (RT * wm + rt) + n;
+        const int r = row0 + 16 * (RT * wave + rt) + n;
         const bool live = r < rows;
         const int seq = live ? r / G : 0;
         const int h = kvh * G + (live ? r % G : 0);
         const float* q = global_ptr(a.seqs[seq].Q) + static_cast<size_t>(h) * D;
-        float x[DC][8];
-        float mx = 0.0f;
+        un_u4 x[DC][2];
 #pragma unroll
         for (int s = 0; s < DC; ++s) {
-            const int c = 32 * s + 8 * g;
-            const bool in = live && c < D;
-            const un_u4 y = *reinterpret_cast<const un_u4*>(q + min(c, D - 8));
-            const un_u4 z = *reinterpret_cast<const un_u4*>(q + min(c, D - 8) + 4);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                x[s][j] = in ? __uint_as_float(y[j]) : 0.0f;
-                x[s][4 + j] = in ? __uint_as_float(z[j]) : 0.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) mx = fmaxf(mx, fabsf(x[s][j]));
+            const int c = min(32 * s + 8 * g, D - 8);
+            x[s][0] = *reinterpret_cast<const un_u4*>(q + c);
+            x[s][1] = *reinterpret_cast<const un_u4*>(q + c + 4);
         }
+        float mx = 0.0f;
+#pragma unroll
+        for (int s = 0; s < DC; ++s)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (!live || 32 * s + 8 * g >= D) x[s][j >> 2][j & 3] = 0u;
+                mx = fmaxf(mx, fabsf(__uint_as_float(x[s][j >> 2][j & 3])));
+            }
         mx = xrow_max(mx);
         const int e = (mx > 0.0f) ? __builtin_amdgcn_frexp_expf(mx) : 0;
 #pragma unroll
@@ -401,289 +994,263 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
             uint2 p[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                p[j] = parts(__builtin_amdgcn_ldexpf(x[s][2 * j], 12 - e), __builtin_amdgcn_ldexpf(x[s][2 * j + 1], 12 - e));
+                p[j] = parts(__builtin_amdgcn_ldexpf(__uint_as_float(x[s][j >> 1][2 * (j & 1)]), 12 - e),
+                             __builtin_amdgcn_ldexpf(__uint_as_float(x[s][j >> 1][2 * (j & 1) + 1]), 12 - e));
             qh[rt][s] = mf_u4{p[0].x, p[1].x, p[2].x, p[3].x};
             ql[rt][s] = mf_u4{p[0].y, p[1].y, p[2].y, p[3].y};
         }
         crow[rt] = __builtin_amdgcn_ldexpf(a.scale2, e - 16);
     }
 
-    mf_f4 acc[RT][2 * DC];
+    mf_f4 acc[RT][2 * DC], d[RT][2];
+    mf_u4 ph[RT], pl[RT];
     float mr[RT], l[RT], pz[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         mr[rt] = -3.0e38f;
         l[rt] = 0.0f;
         pz[rt] = 0.0f;
+        ph[rt] = pl[rt] = mf_u4{0u, 0u, 0u, 0u};
+        d[rt][0] = d[rt][1] = mf_f4{kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
         for (int s = 0; s < 2 * DC; ++s) acc[rt][s] = mf_f4{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    // Exponents of the scales of K and V, and whether no tile has set them yet: of the workgroup, or of each wave
-    // that stages for itself.
-    int k_exp = 0, v_exp = 0;
-    bool kfirst = true, vfirst = true;
-    float* peaks = peak + (C::ALONE ? 2 * wave : 0);
-    if (threadIdx.x < C::PEAKS) peak[threadIdx.x] = 0.0f;
+    // Exponents of the scales of K and V (uniform over the workgroup), and whether no tile has set them yet; that of
+    // the K behind the logits in d.
+    int k_exp = exponent(top.x, 8), v_exp = exponent(top.y, PACKED ? 0 : 8), d_exp = 0;
+    bool kfirst = !__ballot(top.x > 0.0f), vfirst = !__ballot(top.y > 0.0f);
     lds_barrier();
-    auto sync = [&]() {
-        if constexpr (C::ALONE)
-            wave_lds_sync();
-        else
-            lds_barrier();
-    };
+    if (threadIdx.x < 4) peak[threadIdx.x] = 0.0f;
+    // The start multiplies P = 0 with what this buffer holds.
+    for (int x = 16 * threadIdx.x; x < 2 * 32 * DC * L::VS; x += 16 * 64 * WM)
+        *reinterpret_cast<mf_u4*>(lds + ((t0 - 1) & 1) * L::BYTES + L::V + x) = mf_u4{0u, 0u, 0u, 0u};
 
-    // The new exponents that the tile's peaks ask for; true if they changed.
-    auto adjust = [&](const float* pk) -> bool {
-        const float pk_k = pk[0], pk_v = pk[1];
-        int kn = k_exp, vn = v_exp;
-        if (__ballot(pk_k > 0.0f)) {
-            const int e = scalar(__builtin_amdgcn_frexp_expf(pk_k)) - 11;  // largest scaled key below 2^15
-            if (e > k_exp || (kfirst && __ballot(pk_k < kLow))) kn = e;
-            kfirst = false;
-        }
-        if (__ballot(pk_v > 0.0f)) {
-            const int e = scalar(__builtin_amdgcn_frexp_expf(pk_v)) - (PACKED ? 0 : 11);
-            if (e > v_exp + (PACKED ? 1 : 0) || (vfirst && __ballot(pk_v < kLow))) vn = e;
-            vfirst = false;
-        }
-        if (kn == k_exp && vn == v_exp) return false;
-        const float f = __builtin_amdgcn_ldexpf(1.0f, v_exp - vn);
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            pz[rt] *= f;
-#pragma unroll
-            for (int s = 0; s < 2 * DC; ++s) acc[rt][s] *= f;
-        }
-        k_exp = kn;
-        v_exp = vn;
-        return true;
-    };
-
-    // QK of the staged tile.
-    auto qk = [&](const char* tl, mf_f4 (&d)[RT][2]) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) d[rt][i] = mf_f4{0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int s = 0; s < DC; ++s) {
-            mf_u4 kh[2], kl[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const char* p = tl + (16 * i + n) * L::KS + 64 * s + 16 * g;
-                kh[i] = *reinterpret_cast<const mf_u4*>(p + L::KHI);
-                kl[i] = *reinterpret_cast<const mf_u4*>(p + L::KLO);
+    // At the top of the loop K of tile k and V of tile k - 1 are staged. `again`: they have to be, at the start or
+    // with other exponents; nothing is multiplied then (P is zero).
+    int again = 1;
+    asm("" : "+s"(again));  // (or the compiler makes a loop of its own of the start)
+    uint32_t m0 = 0u, m1 = 0u;  // masks of tiles k - 1 and k
+    int k = t0;
+    bool more;
+#pragma unroll 1
+    do {
+        lds_barrier();
+        if (!again || k > t0 || m1) {
+            const float2 pk = *reinterpret_cast<const float2*>(peak + 2 * (k & 1));
+            const float pv_ = peak[2 * ((k - 1) & 1) + 1];
+            int kn = k_exp, vn = v_exp;
+            if (__ballot(pk.x > 0.0f)) {
+                const int e = exponent(pk.x, 8);  // (a peak past the limit asks for at least k_exp + 1 at 11)
+                if (e - 3 > k_exp || kfirst) kn = e;
+                kfirst = false;
             }
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) d[rt][i] = mfma16x16x32(kh[i], ql[rt][s], d[rt][i]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) d[rt][i] = mfma16x16x32(kl[i], qh[rt][s], d[rt][i]);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) d[rt][i] = mfma16x16x32(kh[i], qh[rt][s], d[rt][i]);
-        }
-    };
-    // Softmax of the tile's logits, P (packed: P times V's scale) as the PV A operand.
-    auto softmax = [&](const char* tl, const uint32_t mask, mf_f4 (&d)[RT][2], mf_u4 (&ph)[RT], mf_u4 (&pl)[RT]) {
-        mf_f4 vs[2], vz[2];
-        if constexpr (PACKED) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                vs[i] = *reinterpret_cast<const mf_f4*>(tl + L::VMETA + 64 * i + 16 * g);
-                vz[i] = *reinterpret_cast<const mf_f4*>(tl + L::VMETA + 128 + 64 * i + 16 * g);
+            if (__ballot(pv_ > 0.0f)) {
+                const int e = exponent(pv_, PACKED ? 0 : 8);
+                if (e - (PACKED ? 1 : 3) > v_exp || vfirst) vn = e;
+                vfirst = false;
             }
-        }
-        if (mask != 0xffffffffu) {
+            again = kn != k_exp || vn != v_exp ? 1 : 0;
+            if (again) {
+                const float f = __builtin_amdgcn_ldexpf(1.0f, v_exp - vn);
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+                for (int rt = 0; rt < RT; ++rt) {
+                    pz[rt] *= f;
+                    ph[rt] = pl[rt] = mf_u4{0u, 0u, 0u, 0u};
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const bool in = (mask >> (16 * i + 4 * g + r)) & 1u;
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) d[rt][i][r] = in ? d[rt][i][r] : kNegInf;
+                    for (int s = 0; s < 2 * DC; ++s) acc[rt][s] *= f;
                 }
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const float c = __builtin_amdgcn_ldexpf(crow[rt], k_exp);
-            float mx = fmaxf(fmaxf(fmaxf(d[rt][0][0], d[rt][0][1]), fmaxf(d[rt][0][2], d[rt][0][3])),
-                             fmaxf(fmaxf(d[rt][1][0], d[rt][1][1]), fmaxf(d[rt][1][2], d[rt][1][3])));
-            mx = __builtin_fmaf(mx, c, -kUp);
-            // the reference moves only when a row's maximum passes it by more than the slack
-            if (__ballot(mx > mr[rt] + kSlack)) {
-                mx = xrow_max(mx);
-                const bool up = mx > mr[rt] + kSlack;
-                const float mn = up ? mx : mr[rt];
-                const float al = up ? __builtin_amdgcn_exp2f(mr[rt] - mn) : 1.0f;
-                l[rt] *= al;
-                pz[rt] *= al;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const float ar = __shfl(al, 4 * g + r, 64);
-#pragma unroll
-                    for (int q = 0; q < 2 * DC; ++q) acc[rt][q][r] *= ar;
-                }
-                mr[rt] = mn;
+                k_exp = kn;
+                v_exp = vn;
+                lds_barrier();
             }
-            float p[2][4];
-            float sum = 0.0f;
+        }
+        const int kt = min(again ? k : k + 1, t1 - 1), vt = max(min(again ? k - 1 : k, t1 - 1), t0);
+        fetch_k(kt);
+        fetch_v(vt);
+        const char* kl = lds + (k & 1) * L::BYTES;
+        char* vl = lds + ((k - 1) & 1) * L::BYTES;
+        if (!again) {
+            // Softmax of tile k - 1's logits, P (packed: P times V's scale) as the PV A operand; QK of tile k.
+            if (m0 != 0xffffffffu) {
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    p[i][r] = __builtin_amdgcn_exp2f(__builtin_fmaf(d[rt][i][r], c, -mr[rt]));
-                    sum += p[i][r];
-                    if constexpr (PACKED) {
-                        pz[rt] = __builtin_fmaf(p[i][r], vz[i][r], pz[rt]);
-                        p[i][r] *= vs[i][r];
+                    for (int r = 0; r < 4; ++r) {
+                        const bool in = (m0 >> (16 * i + 4 * g + r)) & 1u;
+#pragma unroll
+                        for (int rt = 0; rt < RT; ++rt) d[rt][i][r] = in ? d[rt][i][r] : kNegInf;
                     }
+            }
+            float c[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+                c[rt] = __builtin_amdgcn_ldexpf(crow[rt], d_exp);
+                float mx = max3(max3(d[rt][0][0], d[rt][0][1], d[rt][0][2]), d[rt][0][3], d[rt][1][0]);
+                mx = max3(mx, max3(d[rt][1][1], d[rt][1][2], d[rt][1][3]), mx);
+                mx = __builtin_fmaf(mx, c[rt], -kUp);
+                // the reference moves only when a row's maximum passes it by more than the slack
+                if (__ballot(mx > mr[rt] + kSlack)) {
+                    mx = xrow_max(mx);
+                    const bool up = mx > mr[rt] + kSlack;
+                    const float mn = up ? mx : mr[rt];
+                    const float al = up ? __builtin_amdgcn_exp2f(mr[rt] - mn) : 1.0f;
+                    l[rt] *= al;
+                    pz[rt] *= al;
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const float ar = __shfl(al, 4 * g + r, 64);
+#pragma unroll
+                        for (int q = 0; q < 2 * DC; ++q) acc[rt][q][r] *= ar;
+                    }
+                    mr[rt] = mn;
                 }
-            l[rt] += sum;
-            const uint2 p0 = parts(p[0][0], p[0][1]), p1 = parts(p[0][2], p[0][3]);
-            const uint2 p2 = parts(p[1][0], p[1][1]), p3 = parts(p[1][2], p[1][3]);
-            ph[rt] = mf_u4{p0.x, p1.x, p2.x, p3.x};
-            pl[rt] = mf_u4{p0.y, p1.y, p2.y, p3.y};
-        }
-    };
-    auto pv = [&](const char* tl, const mf_u4 (&ph)[RT], const mf_u4 (&pl)[RT]) {
+            }
+            mf_f4 dn[RT][2];
 #pragma unroll
-        for (int q = 0; q < 2 * DC; ++q) {
-            const char* p = tl + (16 * q + n) * L::VS + 16 * g;
-            const mf_u4 vh = *reinterpret_cast<const mf_u4*>(p + L::V);
+            for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) acc[rt][q] = mfma16x16x32(pl[rt], vh, acc[rt][q]);
-            if constexpr (!PACKED) {
-                const mf_u4 vl = *reinterpret_cast<const mf_u4*>(p + L::VLO);
+                for (int i = 0; i < 2; ++i) dn[rt][i] = mf_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][q] = mfma16x16x32(ph[rt], vl, acc[rt][q]);
+            for (int s = 0; s < DC; ++s) {
+                mf_u4 kh[2], kw[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const char* p = kl + (16 * i + n) * L::KS + 64 * s + 16 * g;
+                    kh[i] = *reinterpret_cast<const mf_u4*>(p + L::KHI);
+                    kw[i] = *reinterpret_cast<const mf_u4*>(p + L::KLO);
+                }
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) dn[rt][i] = mfma16x16x32(kh[i], ql[rt][s], dn[rt][i]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) dn[rt][i] = mfma16x16x32(kw[i], qh[rt][s], dn[rt][i]);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) dn[rt][i] = mfma16x16x32(kh[i], qh[rt][s], dn[rt][i]);
             }
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) acc[rt][q] = mfma16x16x32(ph[rt], vh, acc[rt][q]);
-        }
-    };
-
-
-    auto stage = [&](char* tl, const uint32_t mask, float* pk) {
-        stage_k(tl, mask, k_exp, kfirst, pk);
-        stage_v(tl, mask, v_exp, vfirst, pk + 1);
-        if constexpr (PACKED)
-            if (vunit(0) == 0) stage_vmeta(tl, mask, v_exp, vfirst, pk + 1);
-    };
-    int buf = 0;
-    for (int tb = t0; tb < t1; tb += WT) {
-        const int tile = tb + wt;
-        const bool mine = tile < t1;
-        char* tl = lds + (C::NBUF * wt + buf) * L::BYTES;
-        float* pk = peaks + 2 * buf;
-        if constexpr (C::NBUF == 1) sync();  // the last tile's readers are done
-        const uint32_t mask = mine ? mask_of(tile) : 0u;
-        if (mine) stage(tl, mask, pk);
-        if (tile + WT < t1) fetch(tile + WT);
-        sync();
-        if (adjust(pk)) {
-            // keys or values outside what f16 holds well at this scale: the tile again
-            sync();
-            if (mine) {
-                fetch(tile);
-                stage(tl, mask, pk);
+            for (int i = 0; i < 2; ++i) {
+                mf_f4 vs, vz;
+                if constexpr (PACKED) {
+                    vs = *reinterpret_cast<const mf_f4*>(vl + L::VMETA + 64 * i + 16 * g);
+                    vz = *reinterpret_cast<const mf_f4*>(vl + L::VMETA + 128 + 64 * i + 16 * g);
+                }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) {
+                    float p[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(d[rt][i][r], c[rt], -mr[rt]));
+                        l[rt] += p[r];
+                        if constexpr (PACKED) {
+                            pz[rt] = __builtin_fmaf(p[r], vz[r], pz[rt]);
+                            p[r] *= vs[r];
+                        }
+                    }
+                    const uint2 x = parts(p[0], p[1]), y = parts(p[2], p[3]);
+                    ph[rt][2 * i] = x.x;
+                    ph[rt][2 * i + 1] = y.x;
+                    pl[rt][2 * i] = x.y;
+                    pl[rt][2 * i + 1] = y.y;
+                    d[rt][i] = dn[rt][i];
+                }
             }
-            if (tile + WT < t1) fetch(tile + WT);
-            sync();
+            interleave<6 * DC * RT>();
+            d_exp = k_exp;
         }
-        if constexpr (C::NBUF == 2) buf ^= 1;
-        if (!mine) continue;
-        mf_f4 d[RT][2];
-        mf_u4 ph[RT], pl[RT];
-        qk(tl, d);
-        softmax(tl, mask, d, ph, pl);
-        pv(tl, ph, pl);
-    }
+        // PV of tile k - 1, and the fetched tiles to LDS.
+        auto pv_and_stage = [&](auto with_k, auto with_v) {
+#pragma unroll
+            for (int q = 0; q < 2 * DC; ++q) {
+                const char* p = vl + (16 * q + n) * L::VS + 16 * g;
+                const mf_u4 vh = *reinterpret_cast<const mf_u4*>(p + L::V);
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt][q] = mfma16x16x32(pl[rt], vh, acc[rt][q]);
+                if constexpr (!PACKED) {
+                    const mf_u4 vw = *reinterpret_cast<const mf_u4*>(p + L::VLO);
+#pragma unroll
+                    for (int rt = 0; rt < RT; ++rt) acc[rt][q] = mfma16x16x32(ph[rt], vw, acc[rt][q]);
+                }
+#pragma unroll
+                for (int rt = 0; rt < RT; ++rt) acc[rt][q] = mfma16x16x32(ph[rt], vh, acc[rt][q]);
+            }
+            const uint32_t mk = mask_of(kt);
+            const uint32_t mv = vt == kt ? mk : (vt == k ? m1 : m0);
+            const int kb = again ? k & 1 : (k + 1) & 1, vb = again ? (k - 1) & 1 : k & 1;
+            float kmx = 0.0f, vmx = 0.0f;
+            if constexpr (decltype(with_k)::value) kmx = stage_k(lds + kb * L::BYTES, mk, k_exp);
+            if constexpr (decltype(with_v)::value) vmx = stage_v(lds + vb * L::BYTES, mv, v_exp);
+            interleave<2 * DC * RT * (PACKED ? 2 : 3)>();
+            if constexpr (decltype(with_k)::value) report(kmx, __builtin_amdgcn_ldexpf(0.0625f, k_exp), kfirst, peak + 2 * kb);
+            if constexpr (decltype(with_v)::value && !PACKED)
+                report(vmx, __builtin_amdgcn_ldexpf(0.0625f, v_exp), vfirst, peak + 2 * vb + 1);
+            if constexpr (decltype(with_v)::value && PACKED) {
+                // a scale up to 2 2^v_exp stays in reach (P <= 2^14): reported in units of kLimit / 2
+                if (has_meta)
+                    report(stage_meta(lds + vb * L::BYTES, mv, v_exp) * (0.5f * kLimit),
+                           __builtin_amdgcn_ldexpf(2.0f / kLimit, v_exp), vfirst, peak + 2 * vb + 1);
+            }
+            if (again) {
+                m1 = mk;
+            } else {
+                m0 = m1;
+                m1 = mk;
+            }
+        };
+        using Yes = std::true_type;
+        using No = std::false_type;
+        if constexpr (EVEN) {
+            pv_and_stage(Yes{}, Yes{});
+        } else if constexpr (APART) {
+            if (has_k)
+                pv_and_stage(Yes{}, No{});
+            else if (WM == 2 * DC || has_v)
+                pv_and_stage(No{}, Yes{});
+            else
+                pv_and_stage(No{}, No{});
+        } else {
+            if (has_k && has_v)
+                pv_and_stage(Yes{}, Yes{});
+            else if (has_k)
+                pv_and_stage(Yes{}, No{});
+            else
+                pv_and_stage(No{}, Yes{});
+        }
+        more = again || k != t1;
+        k += again ? 0 : 1;
+        again = 0;
+    } while (more);
 
-    // The partial in units of V: acc holds 16 V 2^-v_exp (FP32 tiles), or 2 4^(c % 4) of it without the centred zero.
+    // The partial in units of V: acc holds 16 V 2^-v_exp (FP32 tiles), or 2 4^(c % NC) of it without the centred zero.
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) l[rt] = xrow_sum(l[rt]);
-    const float back = __builtin_amdgcn_ldexpf(1.0f, v_exp - (PACKED ? 1 + 2 * (n & 3) : 4));
+    const float back = __builtin_amdgcn_ldexpf(1.0f, v_exp - (PACKED ? 1 + 2 * (n & (NC - 1)) : 4));
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
         const float z = PACKED ? __builtin_amdgcn_ldexpf(xrow_sum(pz[rt]), v_exp) : 0.0f;
+        const int rn = row0 + 16 * (RT * wave + rt) + n;
+        // row rn's partial, behind its sequence's own slots
+        const int seq = rn < rows ? rn / G : 0;
+        const int ns = a.slot_base[seq + 1] - a.slot_base[seq];
+        const int h = kvh * G + (rn < rows ? rn % G : 0);
+        const uint32_t pi = static_cast<uint32_t>(a.slot_base[seq] * a.Hq + h * ns + (ns - a.prefix_slots + slot));
+        if (g == 0 && rn < rows) {
+            a.ml[2 * static_cast<size_t>(pi)] = l[rt] > 0.0f ? mr[rt] : kNegInf;
+            a.ml[2 * static_cast<size_t>(pi) + 1] = l[rt];
+        }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const float zr = PACKED ? __shfl(z, 4 * g + r, 64) : 0.0f;
+            const uint32_t pr = static_cast<uint32_t>(__shfl(static_cast<int>(pi), 4 * g + r, 64));
+            if (row0 + 16 * (RT * wave + rt) + 4 * g + r >= rows) continue;
+            float* o = a.acc + static_cast<size_t>(pr) * D + n;
 #pragma unroll
-            for (int q = 0; q < 2 * DC; ++q) acc[rt][q][r] = __builtin_fmaf(acc[rt][q][r], back, zr);
-        }
-    }
-    auto partial = [&](const int r) {  // index of row r's partial
-        const int seq = r / G;
-        const int h = kvh * G + r % G;
-        const int ns = a.slot_base[seq + 1] - a.slot_base[seq];
-        return static_cast<size_t>(a.slot_base[seq]) * a.Hq + static_cast<size_t>(h) * ns + (ns - a.prefix_slots + slot);
-    };
-    if constexpr (WT == 1) {
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const int rn = row0 + 16 * (RT * wm + rt) + n;
-            if (g == 0 && rn < rows) {
-                const size_t pi = partial(rn);
-                a.ml[2 * pi] = l[rt] > 0.0f ? mr[rt] : kNegInf;
-                a.ml[2 * pi + 1] = l[rt];
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int rr = row0 + 16 * (RT * wm + rt) + 4 * g + r;
-                if (rr >= rows) continue;
-                float* o = a.acc + partial(rr) * D;
-#pragma unroll
-                for (int q = 0; q < 2 * DC; ++q)
-                    if (16 * q < D) o[16 * q + n] = acc[rt][q][r];
-            }
-        }
-    } else {
-        // The waves of one row tile took other tokens: joined in LDS.
-        constexpr int RW = 16 * RT;                 // rows of a wave
-        constexpr int LINE = 32 * DC + 4;           // floats per row: accumulators, reference, sum
-        static_assert(WM * WT * RW * LINE * 4 <= C::TILES * L::BYTES, "the merge fits in the tiles' LDS");
-        lds_barrier();
-        float* my = reinterpret_cast<float*>(lds) + wave * RW * LINE;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            if (g == 0) {
-                my[(16 * rt + n) * LINE + 32 * DC] = mr[rt];
-                my[(16 * rt + n) * LINE + 32 * DC + 1] = l[rt];
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-#pragma unroll
-                for (int q = 0; q < 2 * DC; ++q) my[(16 * rt + 4 * g + r) * LINE + 16 * q + n] = acc[rt][q][r];
-        }
-        lds_barrier();
-        for (int idx = threadIdx.x; idx < WM * RW * 32 * DC; idx += 64 * WM * WT) {
-            const int row = idx / (32 * DC), c = idx - row * 32 * DC;  // row of the workgroup, channel
-            const int rr = row0 + row;
-            if (rr >= rows || c >= D) continue;
-            const float* x = reinterpret_cast<const float*>(lds) + row * LINE;
-            constexpr int STEP = WM * RW * LINE;  // to the next wave of the same rows
-            float M = -3.0e38f;
-#pragma unroll
-            for (int w = 0; w < WT; ++w) M = fmaxf(M, x[w * STEP + 32 * DC]);
-            float A = 0.0f, Ls = 0.0f;
-#pragma unroll
-            for (int w = 0; w < WT; ++w) {
-                const float f = __builtin_amdgcn_exp2f(x[w * STEP + 32 * DC] - M);
-                A = __builtin_fmaf(f, x[w * STEP + c], A);
-                Ls = __builtin_fmaf(f, x[w * STEP + 32 * DC + 1], Ls);
-            }
-            const size_t pi = partial(rr);
-            a.acc[pi * D + c] = A;
-            if (c == 0) {
-                a.ml[2 * pi] = Ls > 0.0f ? M : kNegInf;
-                a.ml[2 * pi + 1] = Ls;
-            }
+            for (int q = 0; q < 2 * DC; ++q)
+                if (16 * q < D) o[16 * q] = __builtin_fmaf(acc[rt][q][r], back, zr);
         }
     }
 }
@@ -696,10 +1263,19 @@ __device__ __forceinline__ int share(const int count, const int i, const int par
 // Grid: slots x (KV heads x row chunks); slot s of all heads and chunks on XCD
 // s % 8, back to back, so that a tile's lines come from memory once. Slots
 // [0, packed_slots) share the packed tiles, the others the FP32 ones.
-template <int DC, int RT, int WM, int WT>
-__global__ void __launch_bounds__(64 * WM * WT) __attribute__((amdgpu_waves_per_eu(Config<DC, RT, WM, WT>::PER_EU)))
+template <int DC, int WM, bool PACKED, typename MetaT>
+__device__ __forceinline__ void any_body(const SharedArgs& a, char* lds, const Tiers& t, const int kvh, const int row0,
+                                         const int rows, const int t0, const int t1, const int slot) {
+    if constexpr (DC > 4)
+        wide_body<DC, 1, WM, PACKED, MetaT>(a, lds, t, kvh, row0, rows, t0, t1, slot);
+    else
+        shared_body<DC, WM, PACKED, MetaT>(a, lds, t, kvh, row0, rows, t0, t1, slot);
+}
+
+template <int DC, int WM, typename MetaT>
+__global__ void __launch_bounds__(64 * WM) __attribute__((amdgpu_waves_per_eu(Config<DC, WM>::PER_EU)))
 attn_shared_kernel(const SharedArgs a) {
-    __shared__ __align__(16) char lds[Config<DC, RT, WM, WT>::LDS];
+    __shared__ __align__(16) char lds[Config<DC, WM>::LDS];
     const unsigned id = blockIdx.x;
     const unsigned q = id >> 3;
     const unsigned hc = static_cast<unsigned>(a.Hkv * a.chunks);
@@ -707,51 +1283,42 @@ attn_shared_kernel(const SharedArgs a) {
     const int s = static_cast<int>((q / hc) * 8 + (id & 7));
     if (s >= a.prefix_slots) return;
     const int kvh = hz / a.chunks, chunk = hz - kvh * a.chunks;
-    const int rows = a.nseq * (a.Hq / a.Hkv), row0 = chunk * 16 * RT * WM;
+    const int rows = a.nseq * (a.Hq / a.Hkv), row0 = chunk * Config<DC, WM>::ROWS;
     const Tiers t = tiers_of(a, kvh);
     if (s < a.packed_slots) {
         const int tiles = (t.slots + kTile - 1) / kTile;
-        shared_body<DC, RT, WM, WT, true>(a, lds, t, kvh, row0, rows, share(tiles, s, a.packed_slots),
-                                          share(tiles, s + 1, a.packed_slots), s);
+        any_body<DC, WM, true, MetaT>(a, lds, t, kvh, row0, rows, share(tiles, s, a.packed_slots),
+                                      share(tiles, s + 1, a.packed_slots), s);
     } else {
         const int tiles = (t.nd + kTile - 1) / kTile, nd = a.prefix_slots - a.packed_slots;
-        shared_body<DC, RT, WM, WT, false>(a, lds, t, kvh, row0, rows, share(tiles, s - a.packed_slots, nd),
-                                           share(tiles, s - a.packed_slots + 1, nd), s);
+        any_body<DC, WM, false, MetaT>(a, lds, t, kvh, row0, rows, share(tiles, s - a.packed_slots, nd),
+                                       share(tiles, s - a.packed_slots + 1, nd), s);
     }
 }
 
-template <int DC, int RT, int WM, int WT>
+template <int DC, int WM>
 int launch(SharedArgs a, const int rows, hipStream_t st) {
-    a.chunks = (rows + 16 * RT * WM - 1) / (16 * RT * WM);
+    a.chunks = (rows + Config<DC, WM>::ROWS - 1) / Config<DC, WM>::ROWS;
     const long long wgs = static_cast<long long>((a.prefix_slots + 7) / 8) * 8 * a.Hkv * a.chunks;
     if (wgs > 0x00ffffffLL) TT_FAIL(TT_ERR_INVALID_ARGUMENT, "attention grid too large");
-    hipLaunchKernelGGL((attn_shared_kernel<DC, RT, WM, WT>), dim3(static_cast<unsigned>(wgs)), dim3(64 * WM * WT), 0, st, a);
+    const dim3 grid(static_cast<unsigned>(wgs));
+    if (a.meta_fp16)
+        hipLaunchKernelGGL((attn_shared_kernel<DC, WM, uint16_t>), grid, dim3(64 * WM), 0, st, a);
+    else
+        hipLaunchKernelGGL((attn_shared_kernel<DC, WM, float>), grid, dim3(64 * WM), 0, st, a);
     TT_LAUNCH_CHECK();
     return TT_OK;
 }
 
-// What a workgroup takes, by rows per KV head and 32-channel chunks of a head:
-// its rows, its tiles at once, and how many workgroups a CU holds.
-struct Shape {
-    int rows, tiles, per_cu;
-};
-enum Size { kOne, kTwo, kFour, kEight };  // row tiles of 32 (kOne: 16), shared by as many waves
-
-Size size_for(const int rows) { return rows <= 16 ? kOne : rows <= 64 ? kTwo : rows <= 128 ? kFour : kEight; }
-
-template <int DC, int RT, int WM, int WT, typename F>
-auto with(F&& f) {
-    return f(std::integral_constant<int, DC>{}, std::integral_constant<int, RT>{}, std::integral_constant<int, WM>{},
-             std::integral_constant<int, WT>{});
-}
+// The instantiation that serves `rows` rows per KV head: 32-channel chunks DC, and four waves or, past their rows, eight.
 template <int DC, typename F>
 auto for_rows(const int rows, F&& f) {
-    constexpr int RT = DC <= 4 ? 2 : 1;
-    switch (size_for(rows)) {
-    case kOne: return with<DC, 1, 1, (DC <= 4 ? 4 : 2)>(f);
-    case kTwo: return with<DC, RT, 2, 2>(f);
-    case kFour: return with<DC, RT, 4, 1>(f);
-    default: return with<DC, RT, 8, 1>(f);
+    using C = std::integral_constant<int, DC>;
+    if constexpr (DC > 4) {
+        return f(C{}, std::integral_constant<int, 8>{});
+    } else {
+        if (rows <= 128) return f(C{}, std::integral_constant<int, 4>{});
+        return f(C{}, std::integral_constant<int, 8>{});
     }
 }
 template <typename F>
@@ -759,14 +1326,17 @@ auto for_shape(const int D, const int rows, F&& f) {
     if (D <= 64) return for_rows<2>(rows, f);
     if (D <= 96) return for_rows<3>(rows, f);
     if (D <= 128) return for_rows<4>(rows, f);
-    if (D <= 192) return for_rows<6>(rows, f);
     return for_rows<8>(rows, f);
 }
 
+// Its rows per workgroup, and the workgroups that a CU holds.
+struct Shape {
+    int rows, per_cu;
+};
 Shape shape_of(const int D, const int rows) {
-    return for_shape(D, rows, [](auto dc, auto rt, auto wm, auto wt) {
-        using C = Config<dc.value, rt.value, wm.value, wt.value>;
-        return Shape{16 * rt.value * wm.value, wt.value, C::PER_CU};
+    return for_shape(D, rows, [](auto dc, auto wm) {
+        using C = Config<dc.value, wm.value>;
+        return Shape{C::ROWS, C::PER_CU};
     });
 }
 
@@ -797,9 +1367,9 @@ SharedPlan shared_plan(const tt_decode_seq& prefix, const tt_decode_seq* seqs, i
         const long long slots = std::max<long long>(1, 256LL * sh.per_cu / groups);
         const double cost = packed + kDenseCost * dense;
         long long np = packed ? std::max<long long>(1, std::llround(slots * packed / cost)) : 0;
-        np = std::min(np, (packed + sh.tiles - 1) / sh.tiles);
+        np = std::min(np, packed);
         long long nd = dense ? std::max<long long>(1, slots - np) : 0;
-        nd = std::min(nd, (dense + sh.tiles - 1) / sh.tiles);
+        nd = std::min(nd, dense);
         p.packed_slots = static_cast<int>(np);
         p.prefix_slots = static_cast<int>(np + nd);
     }
@@ -833,8 +1403,8 @@ int shared_launch(const SharedPlan& plan, const tt_decode_seq& prefix, const tt_
         a.chunks = 1;
         std::memcpy(a.slot_base, b.slot_base, sizeof(a.slot_base));
         const int rows = b.nseq * (Hq / Hkv);
-        const int rc = for_shape(D, rows, [&](auto dc, auto rt, auto wm, auto wt) {
-            return launch<dc.value, rt.value, wm.value, wt.value>(a, rows, stream);
+        const int rc = for_shape(D, rows, [&](auto dc, auto wm) {
+            return launch<dc.value, wm.value>(a, rows, stream);
         });
         if (rc) return rc;
     }
