@@ -200,11 +200,9 @@ __device__ __forceinline__ float max3(const float a, const float b, const float 
     return r;
 }
 
-// Loads from a uniform base at a 32-bit lane offset in bytes. (The offset is opaque, or its 64-bit sum with the base
-// is formed in vector registers.)
+// Loads from a uniform base at a 32-bit lane offset in bytes.
 template <typename T>
-__device__ __forceinline__ T load_at(const void* base, uint32_t off) {
-    asm("" : "+v"(off));
+__device__ __forceinline__ T load_at(const void* base, const uint32_t off) {
     return *reinterpret_cast<const T*>(static_cast<const char*>(base) + off);
 }
 
@@ -267,51 +265,69 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
     uint32_t vx[4][PACKED ? 1 : NC];  // packed: words of 4 tokens; FP32: 4 tokens' channels
     uint2 idv = make_uint2(0u, 0u);
     uint32_t vm = 0u;                 // packed: V scale (lanes 0-31) or zero (lanes 32-63) of token lane % 32
-    // The lane as a value of its own: what is computed from it inside the loop is not kept in registers over it.
-    auto lane_now = [&]() {
-        int x = lane;
+    // A value as one of its own: what is computed from it inside the loop is not kept in registers over it.
+    auto now = [&](auto x) {
         asm volatile("" : "+v"(x));
         return x;
     };
-    auto fetch = [&](const int tile) {
-        const int ln = lane_now();
-        const int s0 = kTile * tile, last = (PACKED ? t.slots : t.nd) - 1 - s0;  // tokens past the last repeat it (they are masked)
-        const uint32_t ck = min(32 * unit + 4 * (ln & 7), D - 4), cv = min(32 * unit + 4 * (ln >> 3), D - 4);
+    // A tile of 32 tokens that passes the end of the tier is read from 32 before it, its tokens of the tile before masked:
+    // so the lanes' offsets from a tile's start are the same for all tiles. (Of a tier shorter than a tile, the tokens
+    // past the last repeat it.)
+    const int total = PACKED ? t.slots : t.nd;
+    auto start_of = [&](const int tile) { return max(min(kTile * tile, total - kTile), 0); };
+    uint32_t o_id = 0u, o_km = 0u, o_vm = 0u, o_k, o_v;  // (those of K and V: the lane's first token)
+    uint32_t k_end = 0u, v_end = 0u;                     // FP32: the last token's
+    {
+        const int last = min(total, kTile) - 1;
+        const uint32_t ck = min(kc, D - 4), cv = min(vc, D - 4);
         if constexpr (PACKED) {
             constexpr uint32_t M = sizeof(MetaT);
-            const uint32_t kw = (min(4 * (ln >> 3), last) >> 4) * stride + ck, km = a.kgs == 32 ? ck : kw;
+            o_id = 8u * min(n, last);
+            o_k = 4u * ((min(4 * ktq, last) >> 4) * stride + ck);
+            o_km = M * (a.kgs == 32 ? ck : o_k / 4u);
+            o_vm = static_cast<uint32_t>(min(n, last)) * a.Hkv * M;
+            o_v = 4u * (min(4 * vtq, last & ~3) * (stride / 16) + (cv >> 4));
+        } else {
+            o_k = 4u * (kt0 * stride + ck);
+            k_end = 4u * (last * stride + ck);
+            o_v = 4u * (4 * vtq * stride + cv + NC * part);
+            v_end = 4u * (last * stride + cv + NC * part);
+        }
+    }
+    auto fetch = [&](const int tile) {
+        const int s0 = start_of(tile);
+        if constexpr (PACKED) {
+            constexpr uint32_t M = sizeof(MetaT);
             const size_t kb = static_cast<size_t>(a.kgs == 32 ? s0 >> 5 : s0 >> 4) * stride * M;
-            idv = load_at<uint2>(t.ids + s0, 8u * min(ln & 31, last));
-            kx[0] = load_at<un_u4>(t.kp + static_cast<size_t>(s0 >> 4) * stride, 4u * kw);
+            idv = load_at<uint2>(t.ids + s0, o_id);
+            kx[0] = load_at<un_u4>(t.kp + static_cast<size_t>(s0 >> 4) * stride, o_k);
             if constexpr (!F16M) {
-                kx[1] = load_at<un_u4>(t.ks + kb, M * km);
-                kx[2] = load_at<un_u4>(t.kz + kb, M * km);
+                kx[1] = load_at<un_u4>(t.ks + kb, o_km);
+                kx[2] = load_at<un_u4>(t.kz + kb, o_km);
             } else {
-                const un_u2 ps = load_at<un_u2>(t.ks + kb, M * km), pz = load_at<un_u2>(t.kz + kb, M * km);
+                const un_u2 ps = load_at<un_u2>(t.ks + kb, o_km), pz = load_at<un_u2>(t.kz + kb, o_km);
                 kx[1] = mf_u4{ps[0], ps[1], pz[0], pz[1]};
             }
             // V's scales in lanes 0-31, its zeros in lanes 32-63
-            const char* from = (ln < 32 ? t.vs : t.vz) + static_cast<size_t>(s0) * a.Hkv * M;
-            vm = *reinterpret_cast<const MetaBits<MetaT>*>(from + static_cast<uint32_t>(min(ln & 31, last)) * a.Hkv * M);
-            const uint32_t words = stride / 16;
+            const char* from = (lane < 32 ? t.vs : t.vz) + static_cast<size_t>(s0) * a.Hkv * M;
+            vm = load_at<MetaBits<MetaT>>(from, o_vm);
+            const size_t words = stride / 16;
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                vx[j][0] = load_at<uint32_t>(t.vp + static_cast<size_t>(s0) * words,
-                                             4u * (min(4 * (ln & 7) + j, last) * words + (cv >> 4)));
+            for (int j = 0; j < 4; ++j) vx[j][0] = load_at<uint32_t>(t.vp + (s0 + j) * words, o_v);
         } else {
+            const float* keys = t.dk + static_cast<size_t>(s0) * stride;
+            const float* values = t.dv + static_cast<size_t>(s0) * stride;
+            const uint32_t ok = now(o_k), ov = now(o_v);
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
-                kx[j] = load_at<un_u4>(t.dk + static_cast<size_t>(s0) * stride,
-                                       4u * (min(4 * (ln >> 3) + NT * part + j, last) * stride + ck));
+            for (int j = 0; j < NT; ++j) kx[j] = load_at<un_u4>(keys, min(ok + 4u * j * stride, k_end));
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float* from = t.dv + static_cast<size_t>(s0) * stride;
-                const uint32_t off = 4u * (min(4 * (ln & 7) + j, last) * stride + cv + NC * part);
+                const uint32_t off = min(ov + 4u * j * stride, v_end);
                 if constexpr (NC == 1) {
-                    vx[j][0] = load_at<uint32_t>(from, off);
+                    vx[j][0] = load_at<uint32_t>(values, off);
                 } else {
                     typedef uint32_t un_nc __attribute__((ext_vector_type(NC), aligned(4)));
-                    const un_nc y = load_at<un_nc>(from, off);
+                    const un_nc y = load_at<un_nc>(values, off);
 #pragma unroll
                     for (int e = 0; e < NC; ++e) vx[j][e] = y[e];
                 }
@@ -320,8 +336,7 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
     };
     // Bit j: token j of the tile is attended (packed: of the K tile in flight).
     auto mask_of = [&](const int tile) -> uint32_t {
-        const int left = (PACKED ? t.slots : t.nd) - kTile * tile;
-        const uint32_t in = left >= 32 ? 0xffffffffu : (1u << left) - 1u;
+        const uint32_t in = total < kTile ? (1u << total) - 1u : 0xffffffffu << (kTile * tile - start_of(tile));
         if constexpr (PACKED) return static_cast<uint32_t>(__ballot((idv.x & idv.y) != 0xffffffffu)) & in;
         return in;
     };
@@ -614,7 +629,7 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
             };
             // Softmax: P (packed: P times V's scale) as the PV A operand.
             if (mask != 0xffffffffu) {
-                const uint32_t mine = mask >> (4 * (lane_now() >> 5));
+                const uint32_t mine = mask >> (4 * (now(lane) >> 5));
 #pragma unroll
                 for (int r = 0; r < 16; ++r) d[r] = ((mine >> (8 * (r >> 2) + (r & 3))) & 1u) ? d[r] : kNegInf;
             }
@@ -631,7 +646,7 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
                 const float al = up ? __builtin_amdgcn_exp2f(mr - mn) : 1.0f;
                 l *= al;
                 pz *= al;
-                const int from = 16 * (lane_now() >> 5);  // bytes: the lane group's first row
+                const int from = 16 * (now(lane) >> 5);  // bytes: the lane group's first row
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     const float ar = __int_as_float(__builtin_amdgcn_ds_bpermute(from + 4 * (8 * (r >> 2) + (r & 3)), __float_as_int(al)));
@@ -696,7 +711,7 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
         a.ml[2 * static_cast<size_t>(pi)] = l > 0.0f ? mr : kNegInf;
         a.ml[2 * static_cast<size_t>(pi) + 1] = l;
     }
-    const int first = 4 * (lane_now() >> 5);
+    const int first = 4 * (now(lane) >> 5);
 #pragma unroll
     for (int r = 0; r < 16; ++r) {
         const int row = 8 * (r >> 2) + first + (r & 3);
