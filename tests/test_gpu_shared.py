@@ -146,6 +146,51 @@ def test_against_64_bits(case):
     run(case)
 
 
+# More sequences than a prefix is read one by one for: tiles of every kind, whole and short, alone and with others.
+MANY = [(hq, hkv, d, b, (pd, pb), ragged, kgs, fp16)
+        for (hq, hkv, d, b) in ((4, 2, 64, 33), (6, 1, 64, 64), (2, 2, 16, 40), (6, 2, 96, 40), (8, 1, 80, 50),
+                                (3, 3, 128, 33), (6, 2, 128, 40), (7, 1, 128, 64), (2, 2, 144, 34), (9, 3, 256, 64))
+        for (pd, pb, kgs, fp16) in ((1, 0, 16, False), (0, 1, 16, True), (31, 0, 16, True), (33, 3, 16, False),
+                                    (64, 1, 32, True), (65, 35, 16, True), (0, 33, 32, False))]
+
+
+@pytest.mark.parametrize("case", MANY, ids=lambda c: str(c[:5] + c[6:]))
+def test_many_sequences_against_64_bits(case):
+    run(case, seed=3, weights=lambda i: i % 16 == 1)
+
+
+@pytest.mark.parametrize("d", [64, 96, 128, 256])
+def test_many_sequences_masks_that_leave_nothing(d):
+    own = lambda i: (0, i % 2)
+    run((8, 2, d, 40, (20, 9), own, 16, False), mask="all")
+    _, batch = run((8, 2, d, 40, (0, 9), own, 16, True), mask="all", weights=lambda i: True)
+    for t in batch:
+        assert bool((t["attn_output"] == 0).all())
+        assert t["mean_attn_weights"] is None or bool((t["mean_attn_weights"] == 0).all())
+
+
+@pytest.mark.parametrize("d", [64, 80, 128, 256])
+@pytest.mark.parametrize("fp16", [False, True])
+def test_first_tiles_that_are_masked_or_tiny(d, fp16):
+    """The scales of the prefix's parts come from its first tiles: these are masked, hold NaN there, or keys and values
+    2^-20 (the FP32 ones' smallest 2^-100) of the later ones'."""
+    def edit(prefix, pref, batch, refs):
+        if not fp16:
+            for x in (prefix["dense_K"], pref[0], prefix["dense_V"], pref[1]):
+                x[:32] *= 2.0 ** -20
+                x[3] *= 2.0 ** -80
+        nd = prefix["dense_count"]
+        prefix["PBS_token_ids"][:64] = -1
+        pref[2][nd:nd + 64] = False
+        prefix["PBS_K_Scales"][:4] = 0x7e00 if fp16 else float("nan")  # FP16 metadata: the bits of NaN, infinity
+        prefix["PBS_V_Zeroes"][:64] = 0x7c00 if fp16 else float("inf")
+        for x in pref[:2]:
+            x[nd:nd + 64] = 0  # not attended
+        return pref, refs
+
+    run((8, 2, d, 40, (80, 40), ragged, 16, fp16), edit=edit)
+
+
 @pytest.mark.parametrize("d,b", [(128, 3), (128, 30), (80, 9), (256, 20)])
 def test_masks_that_leave_nothing(d, b):
     """Every packed slot masked: the FP32 tokens alone; without those, zeros (output and weights)."""

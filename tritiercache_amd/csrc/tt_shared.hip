@@ -33,10 +33,21 @@
 namespace tt {
 namespace {
 
-// Attended tokens of all sequences together (the prefix counted for each) up to
-// which the sequences read the prefix one by one.
-constexpr long long kWalkTokens = 4096;
 constexpr double kDenseCost = 1.5;  // an FP32 tile in packed ones
+
+// What the two ways to attend to a prefix take, in us, to choose between them. Multiplied for all sequences, a fixed part
+// that grows with head_dim (kSharedUs + head_dim / 16), its tiles and its merge; ...
+constexpr double kSharedUs = 14.0;
+constexpr double kMergeRate = 4.5e6;  // bytes per us of partials, written and read
+double tile_us(const int D) { return 2.0 + D / 256.0; }
+// ... read once per sequence, by matrix products (head_dim 128) or the VALU, the launch and the tokens. Fitted to 1 to 32
+// sequences behind 512 to 16k tokens with seven head shapes: the choice is the faster one or within 12% of it in 244
+// of 252 of them. (32/8 heads of 128, whole call, multiplied against read by each: 8 sequences behind 4k 35.5 | 28.0 us,
+// 16 behind 2k 32.7 | 35.6, 16 behind 8k 44 | 60; heads of 64: 4 behind 8k 27.4 | 25.2, 16 behind 4k 27 | 44.)
+double walk_us(const int nseq, const double tokens, const int Hq, const int Hkv, const int D) {
+    if (D == 128) return 11.0 + nseq * Hkv * (0.045 + 0.34e-6 * tokens * D);
+    return 11.0 + 1e-6 * nseq * tokens * D * (0.2 * Hkv + 0.17 * Hq);
+}
 
 constexpr int kTile = 32;           // tokens of a tile: FP32 rows or packed slots
 constexpr float kLimit = 65000.0f;  // scaled keys and values stay below this
@@ -1365,7 +1376,16 @@ SharedPlan shared_plan(const tt_decode_seq& prefix, const tt_decode_seq* seqs, i
     const long long dense = (static_cast<long long>(prefix.dense_count) + kTile - 1) / kTile;
     const long long packed = (static_cast<long long>(prefix.num_blocks) * kgs + kTile - 1) / kTile;
     const long long tokens = static_cast<long long>(prefix.dense_count) + static_cast<long long>(prefix.num_blocks) * kgs;
-    p.per_seq = tokens > 0 && nseq <= kMaxBatchSeqs / 2 && nseq * tokens <= kWalkTokens ? 2 : 1;
+    const Shape sh = shape_of(D, rows);
+    // One round of workgroups, each kind's share by what its tiles cost; fewer where another one's partials cost the merge
+    // more than it saves the others in tiles (32 sequences behind 2k, 32/8 heads of 128: 41.9 -> 37.0 us).
+    const long long groups = static_cast<long long>(Hkv) * ((rows + sh.rows - 1) / sh.rows);
+    const double cost = packed + kDenseCost * dense;
+    const double merge = 8.0 * nseq * Hq * D / kMergeRate;  // us per slot
+    const double best = std::sqrt(tile_us(D) * cost / merge);
+    const long long slots = std::max<long long>(1, std::min<long long>(256LL * sh.per_cu / groups, std::llround(best)));
+    const double shared_us = kSharedUs + D / 16.0 + tile_us(D) * std::ceil(cost / slots) + merge * slots;
+    p.per_seq = tokens > 0 && nseq <= kMaxBatchSeqs / 2 && walk_us(nseq, static_cast<double>(tokens), Hq, Hkv, D) <= shared_us ? 2 : 1;
     tt_decode_seq entries[kMaxBatchSeqs];
     for (int i = 0; i < nseq; ++i) {
         entries[p.per_seq * i] = seqs[i];
@@ -1376,11 +1396,6 @@ SharedPlan shared_plan(const tt_decode_seq& prefix, const tt_decode_seq* seqs, i
     }
     p.entries = own_plan(entries, p.per_seq * nseq, Hq, Hkv, D, kgs, meta_fp16);
     if (p.per_seq == 1 && tokens > 0) {
-        const Shape sh = shape_of(D, rows);
-        const long long groups = static_cast<long long>(Hkv) * ((rows + sh.rows - 1) / sh.rows);
-        // one round of workgroups, each kind's share by what its tiles cost
-        const long long slots = std::max<long long>(1, 256LL * sh.per_cu / groups);
-        const double cost = packed + kDenseCost * dense;
         long long np = packed ? std::max<long long>(1, std::llround(slots * packed / cost)) : 0;
         np = std::min(np, packed);
         long long nd = dense ? std::max<long long>(1, slots - np) : 0;
