@@ -158,6 +158,28 @@ class TriTierCache:
         perm = torch.cat([torch.arange(s, device=device), middle, torch.arange(s + hh, nd, device=device)])
         return ids, perm
 
+    def as_prefix(self):
+        """The tokens the next step attends to, as the prefix of
+        ``_C.fused_attention_decode_shared``: the FP32 tiers joined (sinks, heavy hitters,
+        recent window oldest first) and the packed store as it is. Copies: later calls
+        on this cache leave them as they are."""
+        e = self._engine
+        c = e.counters()
+        s, hh, rw, nb = c["s_count"], c["hh_count"], c["rw_count"], c["pbs_blocks_used"]
+        ring = self._ring(rw, c["rw_head_index"], e.get_S_K().device)
+        out = {"dense_K": torch.cat([e.get_S_K()[:s], e.get_HH_K()[:hh], e.get_RW_K()[ring]]),
+               "dense_V": torch.cat([e.get_S_V()[:s], e.get_HH_V()[:hh], e.get_RW_V()[ring]]),
+               "dense_count": s + hh + rw, "num_blocks": nb}
+        if nb > 0:
+            for name, getter in _PBS_VIEWS.items():
+                rows = nb if name.startswith("PBS_K") else nb * e.chunk_size
+                out[name] = getattr(e, getter)()[:rows].clone()
+        return out
+
+    def _ring(self, rw, head, device):
+        """The recent window's slots, oldest first."""
+        return (torch.arange(rw, device=device) + (head if rw == self.R_size else 0)) % max(rw, 1)
+
     def reconstruct_full_cache(self):
         """(K, V, ids) of every token the next step attends to, dequantised: sinks, then
         heavy hitters and valid packed tokens sorted by token id, then the recent window
@@ -188,7 +210,7 @@ class TriTierCache:
         mids = torch.cat([e.get_HH_token_ids()[:hh], pids[keep]])
         order = torch.argsort(mids)
         mk, mv, mids = mk[order], mv[order], mids[order]
-        ring = (torch.arange(rw, device=dev) + (head if rw == self.R_size else 0)) % max(rw, 1)
+        ring = self._ring(rw, head, dev)
         rk, rv = e.get_RW_K()[ring], e.get_RW_V()[ring]
         rids = torch.arange(total - rw, total, device=dev, dtype=torch.int64)
         sids = torch.arange(s, device=dev, dtype=torch.int64)

@@ -23,6 +23,12 @@ unpatched model; then
   output_attentions=True the step also returns the per-head weights over the
   attended tokens.
 
+With ``FUSED_QK`` set, the q/k norm, the rotation and the casts of a forward that
+records no gradients run in one launch (``_C.qk_norm_rope``) instead of the model
+file's modules: in float32 throughout, rounded once to the model's type (a prompt)
+or not at all (a decode token, whose vectors the engine takes in float32), so the
+results differ from the modules' by their roundings.
+
 There is no path without the engine: a layer whose cache cannot be created
 raises.
 """
@@ -51,6 +57,7 @@ H_RATIO = 0.05
 SCORE_DECAY = 0.999
 K_GROUP_SIZE = 16
 PBS_METADATA_DTYPE = "fp16"
+FUSED_QK = False
 
 # (modeling module, attention class) of every family the patch serves.
 _FAMILIES = (
@@ -108,6 +115,8 @@ def _rotated_qkv(module, hidden_states, position_embeddings):
     q = module.q_proj(hidden_states).view(1, n, hq, d)
     k = module.k_proj(hidden_states).view(1, n, hkv, d)
     v = module.v_proj(hidden_states).view(1, n, hkv, d)
+    if FUSED_QK and _fusable(module, (q, k, v), position_embeddings):
+        return _fused_qkv(module, q, k, v, position_embeddings)
     if getattr(module, "q_norm", None) is not None:
         q = module.q_norm(q)
     if getattr(module, "k_norm", None) is not None:
@@ -120,6 +129,52 @@ def _rotated_qkv(module, hidden_states, position_embeddings):
     else:
         q, k = _rotate_half_rope(q, cos, sin), _rotate_half_rope(k, cos, sin)
     return q, k, v
+
+
+def _fusable(module, qkv, position_embeddings):
+    """Whether ``_C.qk_norm_rope`` computes what the module's norms and rotation do: no gradient is recorded, the
+    rotation is a family's (all of them rotate-half) over whole heads, and the norms are both absent or both the
+    family's own (x / rms * weight, of one epsilon), without hooks."""
+    q = qkv[0]
+    norms = [getattr(module, name, None) for name in ("q_norm", "k_norm")]
+    tables = list(position_embeddings)
+    types = (torch.float32, torch.float16, torch.bfloat16)
+    if norms[0] is None and norms[1] is None:
+        norms = []
+    elif not all(_plain_norm(n, q.shape[-1]) for n in norms) or norms[0].variance_epsilon != norms[1].variance_epsilon:
+        return False
+    weights = [n.weight for n in norms]
+    tensors = [*qkv, *tables, *weights]
+    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
+        return False
+    if any(not t.is_cuda or t.device != q.device or t.dtype not in types for t in tensors):
+        return False
+    if any(t.dtype != x[0].dtype for x in (qkv, tables, weights) for t in x):
+        return False
+    rope = _family_rope(type(module))
+    if rope is not None and rope.__module__ not in [mod for mod, _ in _FAMILIES]:
+        return False
+    n, d = q.shape[1], q.shape[-1]
+    return d % 16 == 0 and d <= 256 and all(t.shape[-1] == d and t.numel() == n * d for t in tables)
+
+
+def _plain_norm(norm, d):
+    return (type(norm).__module__ in [mod for mod, _ in _FAMILIES] and hasattr(norm, "variance_epsilon")
+            and norm.weight.shape == (d,) and not norm._forward_hooks and not norm._forward_pre_hooks)
+
+
+def _fused_qkv(module, q, k, v, position_embeddings):
+    """_rotated_qkv's result from its projections, in one launch; float32 for a decode token."""
+    n = q.shape[1]
+    cos, sin = (t.reshape(n, -1).contiguous() for t in position_embeddings)
+    norm = getattr(module, "q_norm", None)
+    weights = {} if norm is None else {"q_weight": norm.weight.detach(), "k_weight": module.k_norm.weight.detach(),
+                                       "eps": norm.variance_epsilon}
+    step = n == 1
+    qr, kr, vr = _C.qk_norm_rope(q[0].detach(), k[0].detach(), v[0].detach() if step else None, cos, sin,
+                                 out_dtype=torch.float32 if step else q.dtype, **weights)
+    vr = vr[None] if step else v
+    return qr[None].transpose(1, 2), kr[None].transpose(1, 2), vr.transpose(1, 2)
 
 
 def _family_rope(cls):
