@@ -86,6 +86,40 @@ def test_against_the_formula(case):
     assert torch.equal(vo, v.to(dst))
 
 
+@pytest.mark.parametrize("hq,hkv,d,rot,src,dst", [(5, 3, 128, 128, BF16, BF16), (9, 2, 256, 64, F16, BF16),
+                                                  (14, 2, 80, 80, F16, F16), (1, 1, 16, 0, BF16, F16)], ids=str)
+def test_many_tokens_of_16_bits(hq, hkv, d, rot, src, dst):
+    """Views of a joint projection at odd elements, keys and values scattered, as many tokens as several heads of one
+    share a lane group for."""
+    from tritiercache_amd import _C
+
+    tokens = 140000 if d == 16 else 9001
+    g = torch.Generator(device="cuda").manual_seed(d)
+    joint = torch.randn(tokens * (hq + 2 * hkv) * d + 1, generator=g, device="cuda").to(src)[1:]
+    joint = joint.view(tokens, hq + 2 * hkv, d)
+    q, k, v = joint[:, :hq], joint[:, hq:hq + hkv], joint[:, hq + hkv:]
+    cos, sin = tables(500, rot, F32, g) if rot else (None, None)
+    pos = torch.randint(0, 500, (tokens,), generator=g, device="cuda")
+    qw, kw = torch.randn((2, d), generator=g, device="cuda").to(BF16).unbind(0)
+    rows = torch.randperm(tokens + 5, generator=g, device="cuda")[:tokens]
+    rows[::7] = -1
+    tier_k, tier_v = (torch.full((tokens + 5, hkv, d), 7.0, dtype=dst, device="cuda") for _ in range(2))
+    qo, _, _ = _C.qk_norm_rope(q, k, v, cos, sin, pos, qw, kw, rows=rows, k_out=tier_k, v_out=tier_v)
+    at = (cos[pos], sin[pos]) if rot else (None, None)
+    check(qo, *formula(q, qw, *at, 1e-6), "q")
+    z, mag = formula(k, kw, *at, 1e-6)
+    stored = rows >= 0
+    check(tier_k[rows[stored]], z[stored], mag[stored], "k")
+    assert torch.equal(tier_v[rows[stored]], v[stored].to(dst))
+    free = torch.ones(tokens + 5, dtype=torch.bool, device="cuda")
+    free[rows[stored]] = False
+    assert bool((tier_k[free] == 7).all()) and bool((tier_v[free] == 7).all())
+    if src == dst:
+        want = qo.clone()
+        _C.qk_norm_rope(q, k, None, cos, sin, pos, qw, kw, q_out=q, k_out=torch.empty_like(k))
+        assert torch.equal(q, want)
+
+
 @pytest.mark.parametrize("dst", [F32, BF16], ids=str)
 def test_views_positions_and_rows(dst):
     """Views of a joint projection, positions of the sequences' own, rows of a tier: padded tokens and rows outside it
