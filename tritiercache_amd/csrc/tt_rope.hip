@@ -13,7 +13,9 @@
 // rest idle): a lane holds 8 channels of each half of the rotated part, so
 // that both members of a rotated pair sit in one lane, or 16 channels behind
 // it, and the norm's sum crosses lanes of one 16-lane row only. Every element
-// is read and written once, in 16-byte (float32: two 16-byte) accesses.
+// is read and written once, in 16-byte (float32: two 16-byte) accesses: memory
+// is the bound. A prompt of 32k tokens with 32/8 heads of 128 in bfloat16, 805 MB,
+// takes 162 us (5.0 TB/s; a copy of 1 GiB reaches 4.76); few tokens take the launch.
 #include "tt_wave.h"
 
 #include <algorithm>
@@ -202,8 +204,9 @@ int launch_rope(const tt_qk_rope& a, hipStream_t s, const long long min_blocks, 
 }
 
 // Four heads per lane group where that still gives every CU two workgroups, for 16-bit types: of 32/8 heads of 128 in
-// bfloat16, one head and four take 201 | 162 us at 32k tokens, 21.8 | 18.6 at 4096, 7.7 | 8.0 at 1000. (With float32 on
-// either side a lane's stores are 32 bytes apart: at 4096 tokens 29.6 | 40.0 us, and without the caches' part 29.6 | 28.3.)
+// bfloat16, one head and four take 201 | 162 us at 32k tokens, 21.8 | 18.6 at 4096, 7.7 | 8.0 at 1000 (four through the
+// caches: 173, 20.6, 7.8). float32 keeps one head: bfloat16 to float32 takes 29.6 | 40.0 us at 4096 tokens, 61.1 | 80.2 at
+// 8192 (four through the caches: 28.3, 65.1).
 template <typename In, typename Out>
 int launch_rope(const tt_qk_rope& a, hipStream_t s) {
     bool done = false;
