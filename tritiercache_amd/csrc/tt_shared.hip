@@ -489,6 +489,7 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
     }
     // Q' = Q 2^(12 - e), e the exponent of the row's largest value: row n, channels 16 s + 8 h .. + 7.
     const int rn = row0 + 32 * wave + n;
+    const bool rowed = row0 + 32 * wave < rows;  // a wave without rows only stages (and multiplies zeros with K)
     const bool live = rn < rows;
     const int seq = live ? rn / G : 0;
     const int head = kvh * G + (live ? rn % G : 0);
@@ -631,7 +632,7 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
         // (The one place in the loop that fetches: of several, copies would be made, which wait for the loads.)
         fetch(min(ahead, t1 - 1));
         again = again == 2 ? 1 : 0;
-        if (!(skip | again)) {
+        if (rowed && !(skip | again)) {
             mf_u4 vh[2], vw[2];
             auto load_v = [&](const int s) {  // step s: channels 32 (s / 2) .., tokens of half s % 2
                 const char* x = tl + (32 * (s >> 1) + n) * L::VS + 32 * (s & 1) + 16 * h;
@@ -989,6 +990,7 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
 
     // Q' = Q 2^(12 - e), e the exponent of the row's largest value, as the QK B operand: row n of row tile rt, channels
     // 32 s + 8 g .. + 7.
+    const bool rowed = row0 + 16 * RT * wave < rows;  // a wave without rows multiplies nothing (P = 0)
     mf_u4 qh[RT][DC], ql[RT][DC];
     float crow[RT];  // log2 units per unit of the product
 #pragma unroll
@@ -1095,7 +1097,7 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
         fetch_v(vt);
         const char* kl = lds + (k & 1) * L::BYTES;
         char* vl = lds + ((k - 1) & 1) * L::BYTES;
-        if (!again) {
+        if (rowed && !again) {
             // Softmax of tile k - 1's logits, P (packed: P times V's scale) as the PV A operand; QK of tile k.
             if (m0 != 0xffffffffu) {
 #pragma unroll
