@@ -11,18 +11,22 @@
 // The matrix instructions multiply f16, the operator is FP32: every operand is
 // a high and a low f16 part (x = hi + lo to about 21 bits) and a product is
 // hi hi + hi lo + lo hi, summed in FP32.
-//   QK  A = K (16 tokens x 32 channels), B = Q (32 channels x 16 rows):
-//       lane (g = lane / 16, n = lane % 16) receives tokens 4 g .. 4 g + 3 of row n.
-//   PV  A = P (16 rows x 32 tokens), B = V (32 tokens x 16 channels): the two
-//       16-token QK results of a lane are its A operand as they lie, in the
-//       token order k = 8 g + j <-> token 4 g + j (j < 4), 16 + 4 g + j - 4
-//       (else), which V has in LDS.
 // f16 covers 2^-14 .. 2^16 with all its bits, so the parts are scaled by
-// powers of two: Q by its row's largest value (to below 2^12), K and V by 16 and,
-// where a tile holds larger values than 4080 or the first one only values below
-// 1/8, by the exponent that brings them back (k_exp, v_exp; the tile is staged
-// again), P by the running reference m = max - 5 (P <= 2^14 with the slack of
-// the lazy rescale).
+// powers of two: Q by its row's largest value (to below 2^12), K and V by the
+// first tile's (k_exp, v_exp: to 2^11 .. 2^12; a tile with larger values than
+// the limit is staged again with another exponent), P by the running reference
+// m = max - 5 (P <= 2^14 with the slack of the lazy rescale). The codes of
+// packed V are exact in one part, and their scales go into P.
+//
+// Bounds, for 64 sequences behind 32k tokens with 32/8 heads of 128: the
+// products, 34 GFLOP, are 86 with the parts (75 us at the 1149 TFLOP/s that a
+// large f16 product reaches on this card), the prefix's bytes 50 MB (11 us). The
+// prefix takes 106 us: 40% of the cycles are matrix instructions' (at about 2.0
+// GHz), about as many the VALU's, which unpacks, exponentiates and splits P
+// (some 330 instructions per wave and tile of 32 tokens x 32 rows against 40
+// matrix ones), and the two hardly overlap with two waves per SIMD, the most
+// that 230 registers allow. Measured without gain: the two halves of the waves
+// half a tile apart, operands read two steps ahead.
 #include "tt_shared.h"
 #include "tt_wave.h"
 
@@ -49,11 +53,12 @@ double walk_us(const int nseq, const double tokens, const int Hq, const int Hkv,
     return 11.0 + 1e-6 * nseq * tokens * D * (0.2 * Hkv + 0.17 * Hq);
 }
 
+constexpr int kWideDC = 8;          // 32-channel chunks of a head in the kernel for head dims above 128
 constexpr int kTile = 32;           // tokens of a tile: FP32 rows or packed slots
 constexpr float kLimit = 65000.0f;  // scaled keys and values stay below this
-// P's largest value when a row's reference moves, and how much further its
-// logits may rise before it moves again, log2 units: P <= 2^14. (With 12 and 2 a
-// wave of 32 rows rescaled in every other tile.)
+// log2 of P's largest value when a row's reference moves, and how much further
+// its logits may rise before it moves again: P <= 2^14. (With 12 and 2 a wave of
+// 32 rows rescaled in every other tile.)
 constexpr float kUp = 5.0f;
 constexpr float kSlack = 9.0f;
 
@@ -609,7 +614,7 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
         if (!again && __ballot(fmaxf(pk_k, pk_v) > 0.0f)) {
             int kn = k_exp, vn = v_exp;
             if (__ballot(pk_k > 0.0f)) {
-                const int e = exponent(pk_k, 8);  // (a peak past the limit asks for at least k_exp + 1 at 11)
+                const int e = exponent(pk_k, 8);  // (a peak past the limit asks for 4 more at least)
                 if (e - 3 > k_exp || kfirst) kn = e;
                 kfirst = false;
             }
@@ -737,19 +742,19 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
     }
 }
 
-// The same for head dims above 128, whose accumulators leave registers for 16 rows per wave. DC: 32-channel
-// chunks of a head. RT: 16-row tiles per wave. WM: waves, on the same tile with rows of their own.
+// The same for head dims above 128, whose accumulators leave registers for 16 rows per wave. Eight waves,
+// on the same tile with rows of their own.
 //
 // The loop is a pipeline over the tiles: while the matrix cores multiply Q with
 // K of tile k, the VALU turns tile k - 1's logits into P; while they multiply P
 // with V of tile k - 1, it stages K of tile k + 1 and V of tile k, whose loads
 // went out at the top. One barrier per tile.
-template <int DC, int RT, int WM, bool PACKED, typename MetaT>
+template <bool PACKED, typename MetaT>
 __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const Tiers& t, const int kvh,
                                             const int row0, const int rows, const int t0, const int t1,
                                             const int slot) {
+    constexpr int DC = kWideDC, WM = 8;
     using L = TileLds<DC>;
-    static_assert(WM >= DC || WM >= 4, "a K and a V unit per wave at most");
     constexpr bool F16M = sizeof(MetaT) == 2;
     float neg1 = -1.0f;
     asm("" : "+s"(neg1));
@@ -760,25 +765,19 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
     const int G = a.Hq / a.Hkv;
     const int D = a.D;
     const size_t Hkv = static_cast<size_t>(a.Hkv);
-    // A unit is 64 lanes x (4 tokens x 4 channels) of a tile: 32 channels. Where the waves are a multiple of the units,
-    // every wave has a K and a V unit's share (NT tokens, or NC channels, of each lane's); else the first waves stage
-    // K's and, with enough waves, the ones behind them V's, or the last waves backwards.
-    constexpr bool EVEN = WM % DC == 0, APART = !EVEN && WM >= 2 * DC;
-    constexpr int SHARES = EVEN ? WM / DC : 1, NT = 4 / SHARES, NC = 4 / SHARES;
-    const int ku = EVEN ? wave % DC : wave, vu = EVEN ? ku : (APART ? wave - DC : WM - 1 - wave);
-    const int part = EVEN ? wave / DC : 0;
-    const bool has_k = EVEN || ku < DC, has_v = EVEN || (vu >= 0 && vu < DC);
+    // A unit is 64 lanes x (4 tokens x 4 channels) of a tile: 32 channels. Each wave stages one of K and one of V.
+    static_assert(WM == DC, "");
     // K units: lane = (token quad, channel quad); V units the other way round,
     // so that the writes of V's transposed rows spread over the banks.
     const int ktq = lane >> 3, kcq = lane & 7;
     const int vtq = lane & 7, vcq = lane >> 3;
-    const int kc = 32 * ku + 4 * kcq, vc = 32 * vu + 4 * vcq;  // first channels
-    const int kt0 = 4 * ktq + NT * part;                       // first token
-    const bool has_meta = vu == 0 && part == 0;                // stages V's scales and zeros
+    const int kc = 32 * wave + 4 * kcq, vc = 32 * wave + 4 * vcq;  // first channels
+    const int kt0 = 4 * ktq;                                       // first token
+    const bool has_meta = wave == 0;                               // stages V's scales and zeros
 
     // The tile in flight, as it lies in memory.
-    mf_u4 kx[PACKED ? 3 : NT];               // packed: words, scale, zero; FP32: tokens
-    uint32_t vx[4][PACKED ? 1 : NC];         // packed: words of 4 tokens; FP32: 4 tokens' channels
+    mf_u4 kx[PACKED ? 3 : 4];               // packed: words, scale, zero; FP32: tokens
+    uint32_t vx[4][PACKED ? 1 : 4];         // packed: words of 4 tokens; FP32: 4 tokens' channels
     uint2 idv = make_uint2(0u, 0u);
     uint32_t vm = 0u;                        // packed: V scale (lanes 0-31) or zero (lanes 32-63) of token lane % 32
     auto fetch_k = [&](const int tile) {
@@ -787,27 +786,24 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
         if constexpr (PACKED) {
             const int last = t.slots - 1;
             idv = *reinterpret_cast<const uint2*>(t.ids + min(s0 + (lane & 31), last));
-            if (has_k) {
-                const int s = min(s0 + 4 * ktq, last);
-                const size_t km = static_cast<size_t>(a.kgs == 32 ? s >> 5 : s >> 4) * Hkv * D + c;
-                kx[0] = *reinterpret_cast<const un_u4*>(t.kp + static_cast<size_t>(s >> 4) * Hkv * D + c);
-                if constexpr (!F16M) {
-                    kx[1] = *reinterpret_cast<const un_u4*>(t.ks + 4 * km);
-                    kx[2] = *reinterpret_cast<const un_u4*>(t.kz + 4 * km);
-                } else {
-                    const un_u2 ps = *reinterpret_cast<const un_u2*>(t.ks + 2 * km);
-                    const un_u2 pz = *reinterpret_cast<const un_u2*>(t.kz + 2 * km);
-                    kx[1] = mf_u4{ps[0], ps[1], pz[0], pz[1]};
-                }
+            const int s = min(s0 + 4 * ktq, last);
+            const size_t km = static_cast<size_t>(a.kgs == 32 ? s >> 5 : s >> 4) * Hkv * D + c;
+            kx[0] = *reinterpret_cast<const un_u4*>(t.kp + static_cast<size_t>(s >> 4) * Hkv * D + c);
+            if constexpr (!F16M) {
+                kx[1] = *reinterpret_cast<const un_u4*>(t.ks + 4 * km);
+                kx[2] = *reinterpret_cast<const un_u4*>(t.kz + 4 * km);
+            } else {
+                const un_u2 ps = *reinterpret_cast<const un_u2*>(t.ks + 2 * km);
+                const un_u2 pz = *reinterpret_cast<const un_u2*>(t.kz + 2 * km);
+                kx[1] = mf_u4{ps[0], ps[1], pz[0], pz[1]};
             }
-        } else if (has_k) {
+        } else {
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < 4; ++j)
                 kx[j] = *reinterpret_cast<const un_u4*>(t.dk + min(s0 + kt0 + j, t.nd - 1) * Hkv * D + c);
         }
     };
     auto fetch_v = [&](const int tile) {
-        if (!has_v) return;
         const int s0 = kTile * tile;
         const int c = min(vc, D - 4);
         if constexpr (PACKED) {
@@ -822,15 +818,9 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                typedef uint32_t un_nc __attribute__((ext_vector_type(NC), aligned(4)));
-                const float* x = t.dv + min(s0 + 4 * vtq + j, t.nd - 1) * Hkv * D + c + NC * part;
-                if constexpr (NC == 1) {
-                    vx[j][0] = __float_as_uint(*x);
-                } else {
-                    const un_nc y = *reinterpret_cast<const un_nc*>(x);
+                const un_u4 y = *reinterpret_cast<const un_u4*>(t.dv + min(s0 + 4 * vtq + j, t.nd - 1) * Hkv * D + c);
 #pragma unroll
-                    for (int e = 0; e < NC; ++e) vx[j][e] = y[e];
-                }
+                for (int e = 0; e < 4; ++e) vx[j][e] = y[e];
             }
         }
     };
@@ -857,7 +847,7 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
     auto stage_k = [&](char* tl, const uint32_t mask, const int ke) -> float {
         const float ksc = __builtin_amdgcn_ldexpf(16.0f, -ke);
         float mx = 0.0f;
-        float x[NT][4];  // [token][channel]
+        float x[4][4];  // [token][channel]
         if constexpr (PACKED) {
             // no attended token: the block's scale and zero may be anything
             const bool any = ((mask >> (4 * ktq)) & 15u) != 0u && kc < D;
@@ -880,9 +870,9 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
             const uint32_t b = 0x0c0c0400u + 0x0101u * (ktq & 3);
             const uint32_t lo = __builtin_amdgcn_perm(kx[0][1], kx[0][0], b);
             const uint32_t hi = __builtin_amdgcn_perm(kx[0][3], kx[0][2], b);
-            const uint32_t w = (lo | (hi << 16)) >> (2 * NT * part);
+            const uint32_t w = lo | (hi << 16);
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 uint32_t y = (w >> (2 * j)) & 0x03030303u;
                 asm("" : "+v"(y));  // (or every code is extracted by an instruction of its own)
 #pragma unroll
@@ -892,7 +882,7 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
         } else {
             const uint32_t mine = mask >> kt0;
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
                     x[j][e] = ((mine >> j) & 1u) && kc < D ? __uint_as_float(kx[j][e]) * ksc : 0.0f;
@@ -900,7 +890,7 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
                 }
         }
 #pragma unroll
-        for (int j = 0; j < NT; ++j) {
+        for (int j = 0; j < 4; ++j) {
             const uint2 p = parts(x[j][0], x[j][1]), q = parts(x[j][2], x[j][3]);
             char* d = tl + (kt0 + j) * L::KS + 2 * kc;
             *reinterpret_cast<uint2*>(d + L::KHI) = make_uint2(p.x, q.x);
@@ -908,19 +898,19 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
         }
         return mx;
     };
-    // Packed: the centred codes (2 q - 3) 4^(c % NC), exact, of channels c. FP32: f16 parts of V 2^(4 - ve). Token quad vtq
+    // Packed: the centred codes (2 q - 3) 4^(c % 4), exact, of channels c. FP32: f16 parts of V 2^(4 - ve). Token quad vtq
     // sits in the MFMA order: 8 tokens per lane group, its half by the 16-token tile.
     auto stage_v = [&](char* tl, const uint32_t mask, const int ve) -> float {
         float mx = 0.0f;
-        char* d = tl + (vc + NC * part) * L::VS + 16 * (vtq & 3) + 8 * (vtq >> 2);
+        char* d = tl + vc * L::VS + 16 * (vtq & 3) + 8 * (vtq >> 2);
         if constexpr (PACKED) {
             // channels past head_dim hold codes of others, in columns that are not stored
             const uint32_t b = 0x0c040c00u + 0x00010001u * (vcq & 3);
             // the codes of the lane's first channel at bit 1 of each half
-            const uint32_t y0 = (__builtin_amdgcn_perm(vx[1][0], vx[0][0], b) << 1) >> (2 * NC * part);
-            const uint32_t y1 = (__builtin_amdgcn_perm(vx[3][0], vx[2][0], b) << 1) >> (2 * NC * part);
+            const uint32_t y0 = __builtin_amdgcn_perm(vx[1][0], vx[0][0], b) << 1;
+            const uint32_t y1 = __builtin_amdgcn_perm(vx[3][0], vx[2][0], b) << 1;
 #pragma unroll
-            for (int k = 0; k < NC; ++k) {
+            for (int k = 0; k < 4; ++k) {
                 const _Float16 c = static_cast<_Float16>(1024.0f + 3.0f * static_cast<float>(1 << (2 * k)));
                 const mf_h2 off = {c, c};
                 const uint32_t mk = 0x00060006u << (2 * k);
@@ -933,7 +923,7 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
             const float vsc = __builtin_amdgcn_ldexpf(16.0f, -ve);
             const uint32_t mine = (mask >> (4 * vtq)) & 15u;
 #pragma unroll
-            for (int e = 0; e < NC; ++e) {
+            for (int e = 0; e < 4; ++e) {
                 float y[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
@@ -975,27 +965,25 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
             if (has_meta && lane < 32 && ((m >> lane) & 1u)) vmx = fabsf(F16M ? half_lo(vm) : __uint_as_float(vm));
         } else {
 #pragma unroll
-            for (int j = 0; j < NT; ++j)
+            for (int j = 0; j < 4; ++j)
 #pragma unroll
                 for (int e = 0; e < 4; ++e)
                     if (((m >> (kt0 + j)) & 1u) && kc < D) kmx = fmaxf(kmx, fabsf(__uint_as_float(kx[j][e])));
 #pragma unroll
             for (int j = 0; j < 4; ++j)
 #pragma unroll
-                for (int e = 0; e < NC; ++e)
+                for (int e = 0; e < 4; ++e)
                     if (((m >> (4 * vtq + j)) & 1u) && vc < D) vmx = fmaxf(vmx, fabsf(__uint_as_float(vx[j][e])));
         }
         top = group_max<WM>(kmx, vmx, lds, wave, lane);
     }
 
-    // Q' = Q 2^(12 - e), e the exponent of the row's largest value, as the QK B operand: row n of row tile rt, channels
-    // 32 s + 8 g .. + 7.
-    const bool rowed = row0 + 16 * RT * wave < rows;  // a wave without rows multiplies nothing (P = 0)
-    mf_u4 qh[RT][DC], ql[RT][DC];
-    float crow[RT];  // log2 units per unit of the product
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const int r = row0 + 16 * (RT * wave + rt) + n;
+    // Q' = Q 2^(12 - e), e the exponent of the row's largest value, as the QK B operand: row n, channels 32 s + 8 g .. + 7.
+    const bool rowed = row0 + 16 * wave < rows;  // a wave without rows multiplies nothing (P = 0)
+    mf_u4 qh[DC], ql[DC];
+    float crow;  // log2 units per unit of the product
+    {
+        const int r = row0 + 16 * wave + n;
         const bool live = r < rows;
         const int seq = live ? r / G : 0;
         const int h = kvh * G + (live ? r % G : 0);
@@ -1024,25 +1012,19 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
             for (int j = 0; j < 4; ++j)
                 p[j] = parts(__builtin_amdgcn_ldexpf(__uint_as_float(x[s][j >> 1][2 * (j & 1)]), 12 - e),
                              __builtin_amdgcn_ldexpf(__uint_as_float(x[s][j >> 1][2 * (j & 1) + 1]), 12 - e));
-            qh[rt][s] = mf_u4{p[0].x, p[1].x, p[2].x, p[3].x};
-            ql[rt][s] = mf_u4{p[0].y, p[1].y, p[2].y, p[3].y};
+            qh[s] = mf_u4{p[0].x, p[1].x, p[2].x, p[3].x};
+            ql[s] = mf_u4{p[0].y, p[1].y, p[2].y, p[3].y};
         }
-        crow[rt] = __builtin_amdgcn_ldexpf(a.scale2, e - 16);
+        crow = __builtin_amdgcn_ldexpf(a.scale2, e - 16);
     }
 
-    mf_f4 acc[RT][2 * DC], d[RT][2];
-    mf_u4 ph[RT], pl[RT];
-    float mr[RT], l[RT], pz[RT];
+    mf_f4 acc[2 * DC], d[2];
+    mf_u4 ph, pl;
+    float mr = -3.0e38f, l = 0.0f, pz = 0.0f;
+    ph = pl = mf_u4{0u, 0u, 0u, 0u};
+    d[0] = d[1] = mf_f4{kNegInf, kNegInf, kNegInf, kNegInf};
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        mr[rt] = -3.0e38f;
-        l[rt] = 0.0f;
-        pz[rt] = 0.0f;
-        ph[rt] = pl[rt] = mf_u4{0u, 0u, 0u, 0u};
-        d[rt][0] = d[rt][1] = mf_f4{kNegInf, kNegInf, kNegInf, kNegInf};
-#pragma unroll
-        for (int s = 0; s < 2 * DC; ++s) acc[rt][s] = mf_f4{0.0f, 0.0f, 0.0f, 0.0f};
-    }
+    for (int s = 0; s < 2 * DC; ++s) acc[s] = mf_f4{0.0f, 0.0f, 0.0f, 0.0f};
     // Exponents of the scales of K and V (uniform over the workgroup), and whether no tile has set them yet; that of
     // the K behind the logits in d.
     int k_exp = exponent(top.x, 8), v_exp = exponent(top.y, PACKED ? 0 : 8), d_exp = 0;
@@ -1068,7 +1050,7 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
             const float pv_ = peak[2 * ((k - 1) & 1) + 1];
             int kn = k_exp, vn = v_exp;
             if (__ballot(pk.x > 0.0f)) {
-                const int e = exponent(pk.x, 8);  // (a peak past the limit asks for at least k_exp + 1 at 11)
+                const int e = exponent(pk.x, 8);  // (a peak past the limit asks for 4 more at least)
                 if (e - 3 > k_exp || kfirst) kn = e;
                 kfirst = false;
             }
@@ -1080,13 +1062,10 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
             again = kn != k_exp || vn != v_exp ? 1 : 0;
             if (again) {
                 const float f = __builtin_amdgcn_ldexpf(1.0f, v_exp - vn);
+                pz *= f;
+                ph = pl = mf_u4{0u, 0u, 0u, 0u};
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    pz[rt] *= f;
-                    ph[rt] = pl[rt] = mf_u4{0u, 0u, 0u, 0u};
-#pragma unroll
-                    for (int s = 0; s < 2 * DC; ++s) acc[rt][s] *= f;
-                }
+                for (int s = 0; s < 2 * DC; ++s) acc[s] *= f;
                 k_exp = kn;
                 v_exp = vn;
                 lds_barrier();
@@ -1105,39 +1084,32 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
 #pragma unroll
                     for (int r = 0; r < 4; ++r) {
                         const bool in = (m0 >> (16 * i + 4 * g + r)) & 1u;
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt) d[rt][i][r] = in ? d[rt][i][r] : kNegInf;
+                        d[i][r] = in ? d[i][r] : kNegInf;
                     }
             }
-            float c[RT];
+            const float c = __builtin_amdgcn_ldexpf(crow, d_exp);
+            float mx = max3(max3(d[0][0], d[0][1], d[0][2]), d[0][3], d[1][0]);
+            mx = max3(mx, max3(d[1][1], d[1][2], d[1][3]), mx);
+            mx = __builtin_fmaf(mx, c, -kUp);
+            // the reference moves only when a row's maximum passes it by more than the slack
+            if (__ballot(mx > mr + kSlack)) {
+                mx = xrow_max(mx);
+                const bool up = mx > mr + kSlack;
+                const float mn = up ? mx : mr;
+                const float al = up ? __builtin_amdgcn_exp2f(mr - mn) : 1.0f;
+                l *= al;
+                pz *= al;
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                c[rt] = __builtin_amdgcn_ldexpf(crow[rt], d_exp);
-                float mx = max3(max3(d[rt][0][0], d[rt][0][1], d[rt][0][2]), d[rt][0][3], d[rt][1][0]);
-                mx = max3(mx, max3(d[rt][1][1], d[rt][1][2], d[rt][1][3]), mx);
-                mx = __builtin_fmaf(mx, c[rt], -kUp);
-                // the reference moves only when a row's maximum passes it by more than the slack
-                if (__ballot(mx > mr[rt] + kSlack)) {
-                    mx = xrow_max(mx);
-                    const bool up = mx > mr[rt] + kSlack;
-                    const float mn = up ? mx : mr[rt];
-                    const float al = up ? __builtin_amdgcn_exp2f(mr[rt] - mn) : 1.0f;
-                    l[rt] *= al;
-                    pz[rt] *= al;
+                for (int r = 0; r < 4; ++r) {
+                    const float ar = __shfl(al, 4 * g + r, 64);
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const float ar = __shfl(al, 4 * g + r, 64);
-#pragma unroll
-                        for (int q = 0; q < 2 * DC; ++q) acc[rt][q][r] *= ar;
-                    }
-                    mr[rt] = mn;
+                    for (int q = 0; q < 2 * DC; ++q) acc[q][r] *= ar;
                 }
+                mr = mn;
             }
-            mf_f4 dn[RT][2];
+            mf_f4 dn[2];
 #pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) dn[rt][i] = mf_f4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int i = 0; i < 2; ++i) dn[i] = mf_f4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int s = 0; s < DC; ++s) {
                 mf_u4 kh[2], kw[2];
@@ -1148,17 +1120,11 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
                     kw[i] = *reinterpret_cast<const mf_u4*>(p + L::KLO);
                 }
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
+                for (int i = 0; i < 2; ++i) dn[i] = mfma16x16x32(kh[i], ql[s], dn[i]);
 #pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) dn[rt][i] = mfma16x16x32(kh[i], ql[rt][s], dn[rt][i]);
+                for (int i = 0; i < 2; ++i) dn[i] = mfma16x16x32(kw[i], qh[s], dn[i]);
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) dn[rt][i] = mfma16x16x32(kw[i], qh[rt][s], dn[rt][i]);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) dn[rt][i] = mfma16x16x32(kh[i], qh[rt][s], dn[rt][i]);
+                for (int i = 0; i < 2; ++i) dn[i] = mfma16x16x32(kh[i], qh[s], dn[i]);
             }
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -1167,119 +1133,83 @@ __device__ __forceinline__ void wide_body(const SharedArgs& a, char* lds, const 
                     vs = *reinterpret_cast<const mf_f4*>(vl + L::VMETA + 64 * i + 16 * g);
                     vz = *reinterpret_cast<const mf_f4*>(vl + L::VMETA + 128 + 64 * i + 16 * g);
                 }
+                float p[4];
 #pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    float p[4];
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(d[rt][i][r], c[rt], -mr[rt]));
-                        l[rt] += p[r];
-                        if constexpr (PACKED) {
-                            pz[rt] = __builtin_fmaf(p[r], vz[r], pz[rt]);
-                            p[r] *= vs[r];
-                        }
+                for (int r = 0; r < 4; ++r) {
+                    p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(d[i][r], c, -mr));
+                    l += p[r];
+                    if constexpr (PACKED) {
+                        pz = __builtin_fmaf(p[r], vz[r], pz);
+                        p[r] *= vs[r];
                     }
-                    const uint2 x = parts(p[0], p[1]), y = parts(p[2], p[3]);
-                    ph[rt][2 * i] = x.x;
-                    ph[rt][2 * i + 1] = y.x;
-                    pl[rt][2 * i] = x.y;
-                    pl[rt][2 * i + 1] = y.y;
-                    d[rt][i] = dn[rt][i];
                 }
+                const uint2 x = parts(p[0], p[1]), y = parts(p[2], p[3]);
+                ph[2 * i] = x.x;
+                ph[2 * i + 1] = y.x;
+                pl[2 * i] = x.y;
+                pl[2 * i + 1] = y.y;
+                d[i] = dn[i];
             }
-            interleave<6 * DC * RT>();
+            interleave<6 * DC>();
             d_exp = k_exp;
         }
         // PV of tile k - 1, and the fetched tiles to LDS.
-        auto pv_and_stage = [&](auto with_k, auto with_v) {
 #pragma unroll
-            for (int q = 0; q < 2 * DC; ++q) {
-                const char* p = vl + (16 * q + n) * L::VS + 16 * g;
-                const mf_u4 vh = *reinterpret_cast<const mf_u4*>(p + L::V);
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][q] = mfma16x16x32(pl[rt], vh, acc[rt][q]);
-                if constexpr (!PACKED) {
-                    const mf_u4 vw = *reinterpret_cast<const mf_u4*>(p + L::VLO);
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt) acc[rt][q] = mfma16x16x32(ph[rt], vw, acc[rt][q]);
-                }
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) acc[rt][q] = mfma16x16x32(ph[rt], vh, acc[rt][q]);
+        for (int q = 0; q < 2 * DC; ++q) {
+            const char* p = vl + (16 * q + n) * L::VS + 16 * g;
+            const mf_u4 vh = *reinterpret_cast<const mf_u4*>(p + L::V);
+            acc[q] = mfma16x16x32(pl, vh, acc[q]);
+            if constexpr (!PACKED) {
+                const mf_u4 vw = *reinterpret_cast<const mf_u4*>(p + L::VLO);
+                acc[q] = mfma16x16x32(ph, vw, acc[q]);
             }
-            const uint32_t mk = mask_of(kt);
-            const uint32_t mv = vt == kt ? mk : (vt == k ? m1 : m0);
-            const int kb = again ? k & 1 : (k + 1) & 1, vb = again ? (k - 1) & 1 : k & 1;
-            float kmx = 0.0f, vmx = 0.0f;
-            if constexpr (decltype(with_k)::value) kmx = stage_k(lds + kb * L::BYTES, mk, k_exp);
-            if constexpr (decltype(with_v)::value) vmx = stage_v(lds + vb * L::BYTES, mv, v_exp);
-            interleave<2 * DC * RT * (PACKED ? 2 : 3)>();
-            if constexpr (decltype(with_k)::value) report(kmx, __builtin_amdgcn_ldexpf(0.0625f, k_exp), kfirst, peak + 2 * kb);
-            if constexpr (decltype(with_v)::value && !PACKED)
-                report(vmx, __builtin_amdgcn_ldexpf(0.0625f, v_exp), vfirst, peak + 2 * vb + 1);
-            if constexpr (decltype(with_v)::value && PACKED) {
-                // a scale up to 2 2^v_exp stays in reach (P <= 2^14): reported in units of kLimit / 2
-                if (has_meta)
-                    report(stage_meta(lds + vb * L::BYTES, mv, v_exp) * (0.5f * kLimit),
-                           __builtin_amdgcn_ldexpf(2.0f / kLimit, v_exp), vfirst, peak + 2 * vb + 1);
-            }
-            if (again) {
-                m1 = mk;
-            } else {
-                m0 = m1;
-                m1 = mk;
-            }
-        };
-        using Yes = std::true_type;
-        using No = std::false_type;
-        if constexpr (EVEN) {
-            pv_and_stage(Yes{}, Yes{});
-        } else if constexpr (APART) {
-            if (has_k)
-                pv_and_stage(Yes{}, No{});
-            else if (WM == 2 * DC || has_v)
-                pv_and_stage(No{}, Yes{});
-            else
-                pv_and_stage(No{}, No{});
-        } else {
-            if (has_k && has_v)
-                pv_and_stage(Yes{}, Yes{});
-            else if (has_k)
-                pv_and_stage(Yes{}, No{});
-            else
-                pv_and_stage(No{}, Yes{});
+            acc[q] = mfma16x16x32(ph, vh, acc[q]);
         }
+        const uint32_t mk = mask_of(kt);
+        const uint32_t mv = vt == kt ? mk : (vt == k ? m1 : m0);
+        const int kb = again ? k & 1 : (k + 1) & 1, vb = again ? (k - 1) & 1 : k & 1;
+        const float kmx = stage_k(lds + kb * L::BYTES, mk, k_exp);
+        const float vmx = stage_v(lds + vb * L::BYTES, mv, v_exp);
+        interleave<2 * DC * (PACKED ? 2 : 3)>();
+        report(kmx, __builtin_amdgcn_ldexpf(0.0625f, k_exp), kfirst, peak + 2 * kb);
+        if constexpr (!PACKED)
+            report(vmx, __builtin_amdgcn_ldexpf(0.0625f, v_exp), vfirst, peak + 2 * vb + 1);
+        if constexpr (PACKED) {
+            // a scale up to 2 2^v_exp stays in reach (P <= 2^14): reported in units of kLimit / 2
+            if (has_meta)
+                report(stage_meta(lds + vb * L::BYTES, mv, v_exp) * (0.5f * kLimit),
+                       __builtin_amdgcn_ldexpf(2.0f / kLimit, v_exp), vfirst, peak + 2 * vb + 1);
+        }
+        if (!again) m0 = m1;
+        m1 = mk;
         more = again || k != t1;
         k += again ? 0 : 1;
         again = 0;
     } while (more);
 
-    // The partial in units of V: acc holds 16 V 2^-v_exp (FP32 tiles), or 2 4^(c % NC) of it without the centred zero.
+    // The partial in units of V: acc holds 16 V 2^-v_exp (FP32 tiles), or 2 4^(c % 4) of it without the centred zero.
+    l = xrow_sum(l);
+    const float back = __builtin_amdgcn_ldexpf(1.0f, v_exp - (PACKED ? 1 + 2 * (n & 3) : 4));
+    const float z = PACKED ? __builtin_amdgcn_ldexpf(xrow_sum(pz), v_exp) : 0.0f;
+    const int rn = row0 + 16 * wave + n;
+    // row rn's partial, behind its sequence's own slots
+    const int seq = rn < rows ? rn / G : 0;
+    const int ns = a.slot_base[seq + 1] - a.slot_base[seq];
+    const int h = kvh * G + (rn < rows ? rn % G : 0);
+    const uint32_t pi = static_cast<uint32_t>(a.slot_base[seq] * a.Hq + h * ns + (ns - a.prefix_slots + slot));
+    if (g == 0 && rn < rows) {
+        a.ml[2 * static_cast<size_t>(pi)] = l > 0.0f ? mr : kNegInf;
+        a.ml[2 * static_cast<size_t>(pi) + 1] = l;
+    }
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) l[rt] = xrow_sum(l[rt]);
-    const float back = __builtin_amdgcn_ldexpf(1.0f, v_exp - (PACKED ? 1 + 2 * (n & (NC - 1)) : 4));
+    for (int r = 0; r < 4; ++r) {
+        const float zr = PACKED ? __shfl(z, 4 * g + r, 64) : 0.0f;
+        const uint32_t pr = static_cast<uint32_t>(__shfl(static_cast<int>(pi), 4 * g + r, 64));
+        if (row0 + 16 * wave + 4 * g + r >= rows) continue;
+        float* o = a.acc + static_cast<size_t>(pr) * D + n;
 #pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-        const float z = PACKED ? __builtin_amdgcn_ldexpf(xrow_sum(pz[rt]), v_exp) : 0.0f;
-        const int rn = row0 + 16 * (RT * wave + rt) + n;
-        // row rn's partial, behind its sequence's own slots
-        const int seq = rn < rows ? rn / G : 0;
-        const int ns = a.slot_base[seq + 1] - a.slot_base[seq];
-        const int h = kvh * G + (rn < rows ? rn % G : 0);
-        const uint32_t pi = static_cast<uint32_t>(a.slot_base[seq] * a.Hq + h * ns + (ns - a.prefix_slots + slot));
-        if (g == 0 && rn < rows) {
-            a.ml[2 * static_cast<size_t>(pi)] = l[rt] > 0.0f ? mr[rt] : kNegInf;
-            a.ml[2 * static_cast<size_t>(pi) + 1] = l[rt];
-        }
-#pragma unroll
-        for (int r = 0; r < 4; ++r) {
-            const float zr = PACKED ? __shfl(z, 4 * g + r, 64) : 0.0f;
-            const uint32_t pr = static_cast<uint32_t>(__shfl(static_cast<int>(pi), 4 * g + r, 64));
-            if (row0 + 16 * (RT * wave + rt) + 4 * g + r >= rows) continue;
-            float* o = a.acc + static_cast<size_t>(pr) * D + n;
-#pragma unroll
-            for (int q = 0; q < 2 * DC; ++q)
-                if (16 * q < D) o[16 * q] = __builtin_fmaf(acc[rt][q][r], back, zr);
-        }
+        for (int q = 0; q < 2 * DC; ++q)
+            if (16 * q < D) o[16 * q] = __builtin_fmaf(acc[q][r], back, zr);
     }
 }
 
@@ -1295,7 +1225,7 @@ template <int DC, int WM, bool PACKED, typename MetaT>
 __device__ __forceinline__ void any_body(const SharedArgs& a, char* lds, const Tiers& t, const int kvh, const int row0,
                                          const int rows, const int t0, const int t1, const int slot) {
     if constexpr (DC > 4)
-        wide_body<DC, 1, WM, PACKED, MetaT>(a, lds, t, kvh, row0, rows, t0, t1, slot);
+        wide_body<PACKED, MetaT>(a, lds, t, kvh, row0, rows, t0, t1, slot);
     else
         shared_body<DC, WM, PACKED, MetaT>(a, lds, t, kvh, row0, rows, t0, t1, slot);
 }
@@ -1354,7 +1284,7 @@ auto for_shape(const int D, const int rows, F&& f) {
     if (D <= 64) return for_rows<2>(rows, f);
     if (D <= 96) return for_rows<3>(rows, f);
     if (D <= 128) return for_rows<4>(rows, f);
-    return for_rows<8>(rows, f);
+    return for_rows<kWideDC>(rows, f);
 }
 
 // Its rows per workgroup, and the workgroups that a CU holds.
