@@ -100,3 +100,44 @@ def test_python_form():
         _C.fused_attention_decode_shared({"mean_attn_weights": 1}, [], 8, 2, 128)
     with pytest.raises(ValueError):
         _C.fused_attention_decode_shared({}, [], 8, 0, 128)
+
+
+def test_a_tensor_that_is_too_small_is_refused():
+    torch = pytest.importorskip("torch")
+    from tritiercache_amd import _C
+
+    st = _C._Staging(sized=True)
+    with pytest.raises(ValueError, match="'Q' tensor holds 12 bytes, the call needs 16"):
+        st.ptr(torch.zeros(3), "Q", 16)
+    with pytest.raises(ValueError, match="'PBS_K_Scales'"):
+        st.ptr(torch.zeros(8, dtype=torch.float16), "PBS_K_Scales", 32)  # FP16 metadata behind an FP32 call
+
+
+@pytest.mark.gpu
+def test_too_small_tensors_and_prefixes_with_weights_on_the_gpu():
+    torch = pytest.importorskip("torch")
+    from tritiercache_amd import _C
+
+    def seq(**kw):
+        e = {"Q": torch.zeros((8, 64), device="cuda"), "attn_output": torch.full((8, 64), 7.0, device="cuda"),
+             "dense_K": torch.zeros((2, 2, 64), device="cuda"), "dense_V": torch.zeros((2, 2, 64), device="cuda"),
+             "dense_count": 2, "num_blocks": 0}
+        return {**e, **kw}
+
+    pre = {k: v for k, v in seq().items() if k not in ("Q", "attn_output")}
+    for bad in ({"Q": torch.zeros((7, 64), device="cuda")}, {"attn_output": torch.zeros(8, 63, device="cuda")},
+                {"dense_count": 3}, {"Q": torch.zeros((8, 64), dtype=torch.float16, device="cuda")},
+                {"mean_attn_weights": torch.zeros(1, device="cuda")}):
+        good = seq()
+        with pytest.raises(ValueError, match="tensor holds"):
+            _C.fused_attention_decode_shared(pre, [good, seq(**bad)], 8, 2, 64)
+        torch.cuda.synchronize()
+        assert bool((good["attn_output"] == 7).all())
+    with pytest.raises(ValueError, match="tensor holds"):
+        _C.fused_attention_decode_shared({**pre, "dense_count": 9}, [seq()], 8, 2, 64)
+    with pytest.raises(ValueError, match="mean attention weights"):
+        _C.fused_attention_decode_shared({**pre, "mean_attn_weights": torch.zeros(2, device="cuda")}, [seq()], 8, 2, 64)
+    good = seq()
+    _C.fused_attention_decode_shared(pre, [good], 8, 2, 64)
+    torch.cuda.synchronize()
+    assert bool((good["attn_output"] == 0).all())

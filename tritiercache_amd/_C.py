@@ -75,9 +75,10 @@ def _is_fp16(dtype_str: str, scale_obj) -> bool:
 class _Staging:
     """Resolves arguments to device addresses, staging host memory."""
 
-    def __init__(self):
+    def __init__(self, sized=False):
         self._writeback = []
         self._keep = []
+        self._sized = sized  # tensors must hold the bytes that the call reads or writes
 
     def ptr(self, obj, name: str, nbytes: int, writable: bool = False, nullable: bool = False) -> int:
         if obj is None:
@@ -96,6 +97,9 @@ class _Staging:
             if not obj.is_contiguous():
                 raise ValueError(
                     f"Argument '{name}' PyTorch tensor is not contiguous in memory. Call .contiguous() before passing.")
+            if self._sized and obj.numel() * obj.element_size() < nbytes:
+                raise ValueError(f"Argument '{name}' tensor holds {obj.numel() * obj.element_size()} bytes, the call "
+                                 f"needs {nbytes}.")
             if obj.is_cuda:
                 p = obj.data_ptr()
                 if p == 0 and not nullable:
@@ -292,7 +296,7 @@ def fused_attention_decode_shared(prefix, batch, num_q_heads, num_kv_heads, head
     `prefix`: a dict with the tier keys of ``_BATCH_FIELDS`` (dense_K .. num_blocks without Q and the outputs), e.g.
     ``TriTierCache.as_prefix()``. `batch`: the sequences as in fused_attention_decode_batched, each with its own
     tiers behind the prefix (counts of 0 where it has none); mean_attn_weights receives the weights of its own tokens.
-    Attended keys and values and the queries must be finite."""
+    Attended keys and values and the queries must be finite. Runs on the device of the queries."""
     Hq, Hkv, D, kgs = int(num_q_heads), int(num_kv_heads), int(head_dim), int(k_group_size)
     if Hq <= 0 or Hkv <= 0 or D <= 0:
         raise ValueError("num_q_heads, num_kv_heads, and head_dim must be positive integers.")
@@ -303,10 +307,16 @@ def fused_attention_decode_shared(prefix, batch, num_q_heads, num_kv_heads, head
     entries = [dict(e) if isinstance(e, dict) else dict(zip(_BATCH_FIELDS, e)) for e in batch]
     if not entries:
         return
+    q = entries[0].get("Q")
+    with torch.cuda.device(q.device if isinstance(q, torch.Tensor) and q.is_cuda else torch.cuda.current_device()):
+        _decode_shared(pre, entries, Hq, Hkv, D, kgs, pbs_metadata_dtype)
+
+
+def _decode_shared(pre, entries, Hq, Hkv, D, kgs, pbs_metadata_dtype):
     scales = pre.get("PBS_K_Scales")
     fp16 = _is_fp16(pbs_metadata_dtype, scales if scales is not None else entries[0].get("PBS_K_Scales"))
     msz = 2 if fp16 else 4
-    st = _Staging()
+    st = _Staging(sized=True)
     p = _lib.DecodeSeq()
     _fill_tiers(st, p, pre, Hkv, D, kgs, msz)
     seqs = (_lib.DecodeSeq * len(entries))()
@@ -434,6 +444,8 @@ def qk_norm_rope(q, k, v=None, cos=None, sin=None, positions=None, q_weight=None
     rows, k_out and v_out are the caller's. Returns (q_out, k_out, v_out or None)."""
     q = _rows(q, "q")
     tokens, hq, d = q.shape
+    if tokens >= 2 ** 31:
+        raise ValueError(f"Argument 'q' must have fewer than 2^31 tokens, got {tokens}.")
     k = _rows(k, "k", like=q)
     hkv = k.shape[1]
     ins = {"q": q, "k": k}
