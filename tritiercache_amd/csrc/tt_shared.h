@@ -26,8 +26,8 @@ SharedPlan shared_plan(const tt_decode_seq& prefix, const tt_decode_seq* seqs, i
 int shared_launch(const SharedPlan& plan, const tt_decode_seq& prefix, const tt_decode_seq* seqs_dev, int Hq, int Hkv,
                   int D, int kgs, int meta_fp16, void* ws, hipStream_t stream);
 
-// Slots of `n` entries (at most kMaxBatchSeqs), and the launch that fills them.
-BatchPlan own_plan(const tt_decode_seq* entries, int n, int Hq, int Hkv, int D, int kgs, int meta_fp16);
+// Slots of `n` entries (at most kMaxBatchSeqs), per_seq of each sequence, and the launch that fills them.
+BatchPlan own_plan(const tt_decode_seq* entries, int n, int per_seq, int Hq, int Hkv, int D, int kgs, int meta_fp16);
 int own_launch(const SharedPlan& plan, const tt_decode_seq& prefix, const tt_decode_seq* seqs_dev, int Hq, int Hkv,
                int D, int kgs, int meta_fp16, void* ws, hipStream_t stream);
 

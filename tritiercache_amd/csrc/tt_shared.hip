@@ -46,9 +46,10 @@ constexpr double kSharedUs = 14.0;
 constexpr double kMergeRate = 4.5e6;  // bytes per us of partials, written and read
 double tile_us(const int D) { return 2.0 + D / 256.0; }
 // ... read once per sequence, by matrix products (head_dim 128) or the VALU, the launch and the tokens. Fitted to 1 to 32
-// sequences behind 512 to 16k tokens with seven head shapes: the choice is the faster one or within 12% of it in 244
-// of 252 of them. (32/8 heads of 128, whole call, multiplied against read by each: 8 sequences behind 4k 35.5 | 28.0 us,
-// 16 behind 2k 32.7 | 35.6, 16 behind 8k 44 | 60; heads of 64: 4 behind 8k 27.4 | 25.2, 16 behind 4k 27 | 44.)
+// sequences behind 512 to 16k tokens with seven head shapes: the choice is the faster one or within 12% of it in 246 of
+// 252 of them, and 28% slower at worst. (Whole call, multiplied against read by each, 32/8 heads of 128: 8 sequences
+// behind 4k 34.6 | 27.6 us, 16 behind 2k 32.0 | 27.5, 16 behind 8k 43.2 | 50.7, 32 behind 2k 37.0 | 48.4; heads of 64: 4
+// behind 8k 25.6 | 24.7, 16 behind 4k 26.6 | 42.9.)
 double walk_us(const int nseq, const double tokens, const int Hq, const int Hkv, const int D) {
     if (D == 128) return 11.0 + nseq * Hkv * (0.045 + 0.34e-6 * tokens * D);
     return 11.0 + 1e-6 * nseq * tokens * D * (0.2 * Hkv + 0.17 * Hq);
@@ -1327,7 +1328,7 @@ SharedPlan shared_plan(const tt_decode_seq& prefix, const tt_decode_seq* seqs, i
             entries[2 * i + 1].mean_attn_weights = nullptr;
         }
     }
-    p.entries = own_plan(entries, p.per_seq * nseq, Hq, Hkv, D, kgs, meta_fp16);
+    p.entries = own_plan(entries, p.per_seq * nseq, p.per_seq, Hq, Hkv, D, kgs, meta_fp16);
     if (p.per_seq == 1 && tokens > 0) {
         long long np = packed ? std::max<long long>(1, std::llround(slots * packed / cost)) : 0;
         np = std::min(np, packed);

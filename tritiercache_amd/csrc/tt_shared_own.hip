@@ -11,6 +11,8 @@
 namespace tt {
 namespace {
 
+constexpr int kOwnTileCost = 4;  // 16 FP32 tokens in pairs of 16 packed ones, as in the batch's plan
+
 struct OwnArgs {
     const tt_decode_seq* __restrict__ seqs;
     tt_decode_seq prefix;
@@ -155,8 +157,31 @@ int launch_own_split_g(const OwnArgs& b, const int gp, hipStream_t st) {
 
 }  // namespace
 
-BatchPlan own_plan(const tt_decode_seq* entries, int n, int Hq, int Hkv, int D, int kgs, int meta_fp16) {
-    if (use_packed_kernel(D)) return batch_plan(entries, n, Hq, Hkv, D, kgs, meta_fp16);
+BatchPlan own_plan(const tt_decode_seq* entries, int n, int per_seq, int Hq, int Hkv, int D, int kgs, int meta_fp16) {
+    if (use_packed_kernel(D)) {
+        // The batch's plan fills the device once, with at least a slot for each entry and kind of tiers. Where the prefix is
+        // read with many sequences, their few own tokens take most of that, and each prefix is left to a slot: then
+        // three rounds, every slot with about as much to do (24 sequences behind 4k, 28/4 heads: 64.8 -> 34.2 us, 16 behind
+        // 4k, 32/8 heads: 56.6 -> 34.7; 8 behind 8k, which the rule leaves to the batch's plan, 32.1 | 33.0).
+        if (per_seq == 1 || n / 2 * head_chunks(Hq, Hkv) <= 64) return batch_plan(entries, n, Hq, Hkv, D, kgs, meta_fp16);
+        BatchPlan p;
+        p.nseq = n;
+        auto pairs = [&](const int i) { return (static_cast<long long>(entries[i].num_blocks) * (kgs / 16) + 1) / 2; };
+        auto tiles = [&](const int i) { return (static_cast<long long>(entries[i].dense_count) + 15) / 16; };
+        long long total = 0;
+        for (int i = 0; i < n; ++i) total += pairs(i) + kOwnTileCost * tiles(i);
+        const long long budget = std::max<long long>(1, 3LL * 256 / head_chunks(Hq, Hkv));
+        const long long cap = std::max<long long>(16, (total + budget - 1) / budget);
+        for (int i = 0; i < n; ++i) {
+            const int np = static_cast<int>(std::max<long long>(1, (pairs(i) + cap - 1) / cap));
+            const int nd = static_cast<int>((kOwnTileCost * tiles(i) + cap - 1) / cap);
+            p.pk_base[i + 1] = p.pk_base[i] + np;
+            p.dn_base[i + 1] = p.dn_base[i] + nd;
+            p.slot_base[i + 1] = p.slot_base[i] + np + nd;
+        }
+        p.total_slots = p.slot_base[n];
+        return p;
+    }
     // The VALU loop: units of its kind per slot so that all slots make about two rounds of three workgroups per CU, at
     // least one unit for each of a slot's four waves.
     BatchPlan p;
