@@ -159,19 +159,24 @@ int launch_own_split_g(const OwnArgs& b, const int gp, hipStream_t st) {
 
 BatchPlan own_plan(const tt_decode_seq* entries, int n, int per_seq, int Hq, int Hkv, int D, int kgs, int meta_fp16) {
     if (use_packed_kernel(D)) {
-        // The batch's plan fills the device once, with at least a slot for each entry and kind of tiers. Where the prefix is
-        // read with many sequences, their few own tokens take most of that, and each prefix is left to a slot: then
-        // three rounds, every slot with about as much to do (24 sequences behind 4k, 28/4 heads: 64.8 -> 34.2 us, 16 behind
-        // 4k, 32/8 heads: 56.6 -> 34.7; 8 behind 8k, which the rule leaves to the batch's plan, 32.1 | 33.0).
-        if (per_seq == 1 || n / 2 * head_chunks(Hq, Hkv) <= 64) return batch_plan(entries, n, Hq, Hkv, D, kgs, meta_fp16);
+        if (per_seq == 1) return batch_plan(entries, n, Hq, Hkv, D, kgs, meta_fp16);
+        // The batch's plan fills the device once, with eight units (a pair of packed 16-token words each) or more per slot.
+        // Where the prefix is read with many sequences, their few own tokens take most of that, and each prefix is left to
+        // a slot: then three rounds, every slot with about as much to do (24 sequences behind 4k, 28/4 heads: 64.8 ->
+        // 34.2 us, 16 behind 4k, 32/8 heads: 56.6 -> 34.7; 8 behind 8k, which are left to the batch's plan, 32.1 | 33.0).
+        // And where there is little to do, slots of four units (2 sequences behind 580, 32/8 heads: 13.3 -> 11.7 us, 1
+        // behind 2048 14.0 -> 12.6; 8 behind 580 13.5 | 16.8).
         BatchPlan p;
         p.nseq = n;
         auto pairs = [&](const int i) { return (static_cast<long long>(entries[i].num_blocks) * (kgs / 16) + 1) / 2; };
         auto tiles = [&](const int i) { return (static_cast<long long>(entries[i].dense_count) + 15) / 16; };
         long long total = 0;
         for (int i = 0; i < n; ++i) total += pairs(i) + kOwnTileCost * tiles(i);
+        const int heads = n / 2 * head_chunks(Hq, Hkv);
         const long long budget = std::max<long long>(1, 3LL * 256 / head_chunks(Hq, Hkv));
-        const long long cap = std::max<long long>(16, (total + budget - 1) / budget);
+        const bool little = heads <= 32 && total < 8 * budget;
+        if (!little && heads <= 64) return batch_plan(entries, n, Hq, Hkv, D, kgs, meta_fp16);
+        const long long cap = std::max<long long>(little ? 4 : 16, (total + budget - 1) / budget);
         for (int i = 0; i < n; ++i) {
             const int np = static_cast<int>(std::max<long long>(1, (pairs(i) + cap - 1) / cap));
             const int nd = static_cast<int>((kOwnTileCost * tiles(i) + cap - 1) / cap);
