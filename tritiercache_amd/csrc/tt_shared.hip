@@ -105,14 +105,15 @@ struct SharedArgs {
     int slot_base[kMaxBatchSeqs + 1];
 };
 
-// (hi, lo) of two values, both truncated: hi + lo is x to 21 bits. `neg1` is -1
-// whose value the compiler does not know: the remainder is then one mixed fused
-// multiply-add instead of a conversion and a subtraction.
+// (hi, lo) of two values, both rounded to nearest: hi + lo is x to 23 bits, off to either side (truncated parts would make
+// every product too small, and the prefix's weights with it). `neg1` is -1 whose value the compiler does not know: the
+// remainder is then one mixed fused multiply-add instead of a conversion and a subtraction.
 __device__ __forceinline__ uint2 parts(const float x0, const float x1, const float neg1) {
-    const auto hi = __builtin_amdgcn_cvt_pkrtz(x0, x1);
-    const mf_h2 h = __builtin_bit_cast(mf_h2, hi);
-    const float r0 = __builtin_fmaf(static_cast<float>(h.x), neg1, x0), r1 = __builtin_fmaf(static_cast<float>(h.y), neg1, x1);
-    return make_uint2(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(r0, r1)));
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const mf_h2 hi = __builtin_convertvector((f2{x0, x1}), mf_h2);
+    const float r0 = __builtin_fmaf(static_cast<float>(hi.x), neg1, x0), r1 = __builtin_fmaf(static_cast<float>(hi.y), neg1, x1);
+    const mf_h2 lo = __builtin_convertvector((f2{r0, r1}), mf_h2);
+    return make_uint2(__builtin_bit_cast(uint32_t, hi), __builtin_bit_cast(uint32_t, lo));
 }
 
 // The exponent of the scale for keys and values up to `peak` (0: not known): 16 peak 2^-e in 2^11 .. 2^12 for `below` = 8, which
