@@ -253,8 +253,10 @@ TT_API int tt_fused_attention_decode_batched(const tt_decode_seq* seqs, const tt
 /* Decode of a batch whose sequences share a prefix (a common system prompt or
  * document): sequence i attends to the prefix's tokens and to its own, in one
  * softmax over both; the prefix's tiers are read once for all sequences and
- * multiplied with all their queries. No counterpart in the reference, whose
- * callers hold the prefix in every sequence's cache (bindings.cpp:99-178).
+ * multiplied with all their queries, or (a short prefix, or few sequences) read
+ * for each sequence in the launch of its own tiers, whichever takes less time.
+ * No counterpart in the reference, whose callers hold the prefix in every
+ * sequence's cache (bindings.cpp:99-178).
  *
  * `prefix` (host memory): the tiers and counts of the shared tokens, shared by
  * every sequence and only read; its Q and attn_output are not used and its

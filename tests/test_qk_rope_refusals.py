@@ -102,3 +102,14 @@ def test_struct_layout_matches_the_header(tmp_path):
     subprocess.run(["gcc", "-I", inc, str(src), "-o", str(tmp_path / "layout")], check=True)
     got = subprocess.run([str(tmp_path / "layout")], capture_output=True, text=True, check=True).stdout.split()
     assert [int(x) for x in got] == [C.sizeof(_lib.QkRope)] + [getattr(_lib.QkRope, n).offset for n in names]
+
+
+def test_inputs_that_record_gradients_are_refused():
+    from tritiercache_amd import _C
+
+    q, k, w = torch.zeros(2, 4, 64), torch.zeros(2, 2, 64), torch.ones(64)
+    for name in ("q", "k", "v", "q_weight", "q_out"):
+        given = {"q": q, "k": k, "v": k.clone(), "q_weight": w, "q_out": q.clone()}
+        given[name] = given[name].clone().requires_grad_()
+        with pytest.raises(ValueError, match="no backward pass"):
+            _C.qk_norm_rope(**given)

@@ -290,8 +290,8 @@ def fused_attention_decode_batched(batch, num_q_heads, num_kv_heads, head_dim, k
 def fused_attention_decode_shared(prefix, batch, num_q_heads, num_kv_heads, head_dim, k_group_size=16,
                                   pbs_metadata_dtype="fp32"):
     """One decode step of sequences that share a prefix (a common system prompt or document): every sequence attends
-    to the prefix's tokens and its own in one softmax, and the prefix's tiers are read once for all of them. No
-    counterpart in the reference.
+    to the prefix's tokens and its own in one softmax, and the prefix is unpacked and multiplied once for all of them
+    (a short one, or that of few sequences, once for each). No counterpart in the reference.
 
     `prefix`: a dict with the tier keys of ``_BATCH_FIELDS`` (dense_K .. num_blocks without Q and the outputs), e.g.
     ``TriTierCache.as_prefix()``. `batch`: the sequences as in fused_attention_decode_batched, each with its own
@@ -441,7 +441,8 @@ def qk_norm_rope(q, k, v=None, cos=None, sin=None, positions=None, q_weight=None
     the token's queries and keys NaN). q_weight, k_weight [head_dim]: weights of the RMS norms, None for no norm.
     rows [tokens] int64: the row of k_out and v_out that takes the token's keys and values (None: row t; -1 or any
     row that is not there: not stored). Outputs that are not given are allocated in out_dtype (q's type where that is None); with
-    rows, k_out and v_out are the caller's. Returns (q_out, k_out, v_out or None)."""
+    rows, k_out and v_out are the caller's. No backward pass: inputs that record gradients are refused. Returns (q_out, k_out,
+    v_out or None)."""
     q = _rows(q, "q")
     tokens, hq, d = q.shape
     if tokens >= 2 ** 31:
@@ -480,6 +481,9 @@ def qk_norm_rope(q, k, v=None, cos=None, sin=None, positions=None, q_weight=None
             raise ValueError("q_weight and k_weight must be contiguous [head_dim] tensors of one type.")
     if rows is not None and (k_out is None or (v is not None and v_out is None)):
         raise ValueError("with rows, k_out and v_out are the caller's tensors.")
+    if torch.is_grad_enabled() and any(isinstance(x, torch.Tensor) and x.requires_grad
+                                       for x in (q, k, v, cos, sin, q_weight, k_weight, q_out, k_out, v_out)):
+        raise ValueError("qk_norm_rope has no backward pass: call it under torch.no_grad() or on detached tensors.")
     _require_gpu()
     odt = out_dtype
     if odt is None:
