@@ -25,7 +25,10 @@ namespace {
 
 typedef __bf16 bf16_t;
 
-// Eight consecutive values as they lie in memory. A row starts at a multiple
+// Eight consecutive values as they lie in memory, stored past the caches (cold
+// buffers, 32/8 heads of 128, through them and past them: bfloat16 to float32
+// at 1777 tokens 19.9 | 16.3 us, at 8192 68.4 | 63.5; float32 to float32 21.7 |
+// 20.4, 76.3 | 76.8; bfloat16 to bfloat16 with four heads at 32k 173 | 162). A row starts at a multiple
 // of its element's size only: the types say so, and the hardware takes any.
 template <typename T>
 struct Eight;
@@ -45,8 +48,8 @@ struct Eight<float> {
             b[j - 4] = x;
     }
     __device__ __forceinline__ void store(float* p) const {
-        *reinterpret_cast<v4*>(p) = a;
-        *reinterpret_cast<v4*>(p + 4) = b;
+        __builtin_nontemporal_store(a, reinterpret_cast<v4*>(p));
+        __builtin_nontemporal_store(b, reinterpret_cast<v4*>(p + 4));
     }
 };
 template <typename T>
@@ -56,8 +59,7 @@ struct Eight {
     __device__ __forceinline__ void load(const T* p) { a = *reinterpret_cast<const v8*>(p); }
     __device__ __forceinline__ float get(const int j) const { return static_cast<float>(a[j]); }
     __device__ __forceinline__ void set(const int j, const float x) { a[j] = static_cast<T>(x); }  // to nearest even
-    __device__ __forceinline__ void store(T* p) const { *reinterpret_cast<v8*>(p) = a; }
-    __device__ __forceinline__ void store_past(T* p) const { __builtin_nontemporal_store(a, reinterpret_cast<v8*>(p)); }
+    __device__ __forceinline__ void store(T* p) const { __builtin_nontemporal_store(a, reinterpret_cast<v8*>(p)); }
 };
 
 template <typename T>
@@ -78,8 +80,7 @@ __device__ __forceinline__ void load8(const void* p, const int64_t i, const int 
 }
 
 // NH: heads of one token that a lane group takes one after another, with the
-// token's row of the tables in registers and the loads of all of them in
-// flight; four write past the caches.
+// token's row of the tables in registers and the loads of all of them in flight.
 template <typename In, typename Out, int NH>
 __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const tt_qk_rope a, const int lanes_log2,
                                                            const int chunks_q, const int chunks_kv, const int chunks) {
@@ -176,13 +177,8 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const tt_qk_rope a, c
             }
         }
         if (on && stored && h0 + i < heads) {
-            if constexpr (NH > 1) {
-                z0.store_past(dst + (h0 + i) * ohs + lo);
-                z1.store_past(dst + (h0 + i) * ohs + hi);
-            } else {
-                z0.store(dst + (h0 + i) * ohs + lo);
-                z1.store(dst + (h0 + i) * ohs + hi);
-            }
+            z0.store(dst + (h0 + i) * ohs + lo);
+            z1.store(dst + (h0 + i) * ohs + hi);
         }
     }
 }
@@ -204,9 +200,8 @@ int launch_rope(const tt_qk_rope& a, hipStream_t s, const long long min_blocks, 
 }
 
 // Four heads per lane group where that still gives every CU two workgroups, for 16-bit types: of 32/8 heads of 128 in
-// bfloat16, one head and four take 201 | 162 us at 32k tokens, 21.8 | 18.6 at 4096, 7.7 | 8.0 at 1000 (four through the
-// caches: 173, 20.6, 7.8). float32 keeps one head: bfloat16 to float32 takes 29.6 | 40.0 us at 4096 tokens, 61.1 | 80.2 at
-// 8192 (four through the caches: 28.3, 65.1).
+// bfloat16, one head and four take 191 | 162 us at 32k tokens, 21.7 | 18.6 at 4096, 7.9 | 8.0 at 1000. float32 keeps one
+// head: bfloat16 to float32 takes 32.7 | 40.0 us at 4096 tokens, 61.5 | 80.2 at 8192.
 template <typename In, typename Out>
 int launch_rope(const tt_qk_rope& a, hipStream_t s) {
     bool done = false;
