@@ -382,3 +382,56 @@ def test_many_sequences_on_two_streams_with_a_workspace_each():
     torch.cuda.synchronize()
     for x in (batch, other):
         assert all(torch.equal(t["attn_output"], y) for t, y in zip(x, want))
+
+
+@pytest.mark.parametrize("d", [64, 128, 256])
+@pytest.mark.parametrize("b", [3, 40])
+@pytest.mark.parametrize("fp16", [False, True])
+def test_tiers_at_any_element(d, b, fp16):
+    """Tiers that begin at the second element of their memory: no alignment but the element's."""
+    def moved(x):
+        y = torch.empty(x.numel() + 1, dtype=x.dtype, device="cuda")[1:].view(x.shape)
+        y.copy_(x)
+        return y
+
+    def edit(prefix, pref, batch, refs):
+        for t in [prefix, *batch]:
+            for k in KEYS + ("Q", "attn_output", "mean_attn_weights"):
+                if isinstance(t.get(k), torch.Tensor) and t[k].numel():
+                    t[k] = moved(t[k])
+        return pref, refs
+
+    run((8, 2, d, b, (70, 13), ragged, 16, fp16), seed=8, edit=edit)
+
+
+@pytest.mark.parametrize("b", [2, 40])
+def test_a_long_fp32_prefix(b):
+    """FP32 tiers of more than 4 GiB: zeros (logits 0, values 0) but for the last tokens, so that a sequence's output is
+    sum e^s v / (zeros + sum e^s) over those."""
+    from tritiercache_amd import _C
+
+    hq, hkv, d, nd, tail = 32, 32, 256, 131072 + 333, 37
+    g = torch.Generator(device="cuda").manual_seed(16)
+    K, V = (torch.zeros((nd, hkv, d), device="cuda") for _ in range(2))
+    K[-tail:] = torch.randn((tail, hkv, d), generator=g, device="cuda")
+    V[-tail:] = torch.randn((tail, hkv, d), generator=g, device="cuda")
+    q = torch.randn((b, hq, d), generator=g, device="cuda") * 3
+    out = torch.empty((b, hq, d), device="cuda")
+    batch = [{"Q": q[i], "attn_output": out[i], "dense_count": 0, "num_blocks": 0} for i in range(b)]
+    _C.fused_attention_decode_shared({"dense_K": K, "dense_V": V, "dense_count": nd, "num_blocks": 0}, batch, hq, hkv, d)
+    torch.cuda.synchronize()
+    k, v = K[-tail:].double().transpose(0, 1), V[-tail:].double().transpose(0, 1)  # [heads, tail, D]
+    for i in range(b):
+        x = q[i].double()[:, None]
+        s = (x @ k.transpose(1, 2))[:, 0] / d ** 0.5
+        size = (x.abs() @ k.abs().transpose(1, 2))[:, 0] / d ** 0.5
+        w = torch.exp(s) / (nd - tail + torch.exp(s).sum(-1, keepdim=True))
+        off = (3 * 2.0 ** -20 + 56 * 2.0 ** -24) * size + 2.0 ** -23 * s.abs()
+        rel = 2 * off.amax(-1, keepdim=True) + 2.0 ** -15  # as in expected()
+        want, mag = (w[:, None] @ v)[:, 0], (w[:, None] @ v.abs())[:, 0]
+        assert bool(((out[i].double() - want).abs() <= (rel + 3 * 2.0 ** -20) * mag + 2.0 ** -126).all()), i
+
+
+def test_more_rows_than_a_workgroup_takes():
+    """128 query heads of one KV head, 64 sequences: 8192 rows."""
+    run((128, 1, 64, 64, (70, 21), lambda i: (1 + i % 3, i % 2), 16, False), seed=9, weights=lambda i: i == 5)
