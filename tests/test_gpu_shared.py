@@ -435,3 +435,38 @@ def test_a_long_fp32_prefix(b):
 def test_more_rows_than_a_workgroup_takes():
     """128 query heads of one KV head, 64 sequences: 8192 rows."""
     run((128, 1, 64, 64, (70, 21), lambda i: (1 + i % 3, i % 2), 16, False), seed=9, weights=lambda i: i == 5)
+
+
+# Few rows behind long prefixes: a wave's tiles are its own. Tiles that start and end anywhere, both kinds, masked ones.
+LONG = [(8, 8, 128, 3, (1000, 3001), ragged, 16, True), (32, 8, 64, 8, (33, 1100), ragged, 32, False),
+        (32, 32, 80, 5, (700, 250), lambda i: (i, i % 2), 16, True), (12, 12, 96, 32, (1, 600), lambda i: (i % 7, 0), 16, False),
+        (32, 32, 16, 9, (5, 501), lambda i: (i, 0), 16, True), (28, 4, 128, 4, (0, 3500), ragged, 16, False),
+        (16, 16, 112, 2, (2500, 400), lambda i: (0, i), 32, True), (4, 1, 128, 8, (12000, 0), ragged, 16, False)]
+
+
+@pytest.mark.parametrize("case", LONG, ids=lambda c: str(c[:5] + c[6:]))
+def test_few_rows_behind_a_long_prefix(case):
+    run(case, seed=21, weights=lambda i: i % 4 == 1)
+
+
+@pytest.mark.parametrize("d", [64, 80, 128])
+@pytest.mark.parametrize("fp16", [False, True])
+def test_few_rows_masked_first_tiles_and_sizes(d, fp16):
+    """Masked first tiles with NaN scales, then tiles a thousand times larger than those before them."""
+    def edit(prefix, pref, batch, refs):
+        nd = prefix["dense_count"]
+        prefix["PBS_token_ids"][:64] = -1
+        pref[2][nd:nd + 64] = False
+        prefix["PBS_K_Scales"][:4] = 0x7e00 if fp16 else float("nan")
+        prefix["PBS_V_Zeroes"][:64] = 0x7c00 if fp16 else float("inf")
+        for x in pref[:2]:
+            x[nd:nd + 64] = 0  # not attended
+        for x, r in ((prefix["dense_K"], pref[0]), (prefix["dense_V"], pref[1])):
+            for at, f in ((100, 1e3), (101, 1e6), (150, 1e9)):
+                x[at:] *= f
+                r[at:nd] *= f
+        for t in batch:
+            t["Q"] *= 1e-18
+        return pref, refs
+
+    run((8, 8, d, 6, (200, 3000), ragged, 16, fp16), seed=22, edit=edit, weights=lambda i: i % 4 == 1)

@@ -1,5 +1,5 @@
 """Register budget of the kernels of a shared prefix and of the head norms with rotation (CPU: compiles the device code
-only): no instantiation spills, and the prefix's kernel keeps two waves per SIMD, which its rounds of workgroups count on."""
+only): no instantiation spills, and the prefix's kernels keep the waves per SIMD that their rounds of workgroups count on."""
 import os
 import re
 import subprocess
@@ -31,6 +31,7 @@ def compiled(name, out):
 
 @pytest.mark.parametrize("source,kernel,count,waves", [
     ("tt_shared.hip", "attn_shared_kernel", 14, 2),  # head dims 64, 96, 128 with 4 or 8 waves and 256, FP32 and FP16 metadata
+    ("tt_shared.hip", "attn_shared_few_kernel", 6, 1),  # head dims 64, 96, 128, FP32 and FP16 metadata
     ("tt_rope.hip", "qk_norm_rope_kernel", 13, 4),   # nine pairs of types, four of 16 bits with four heads too
 ])
 def test_no_spills(tmp_path, source, kernel, count, waves):

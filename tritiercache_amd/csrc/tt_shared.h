@@ -18,6 +18,7 @@ struct SharedPlan {
     int per_seq = 1;
     int prefix_slots = 0;    // of which the first packed_slots share the packed tiles, the others the FP32 ones
     int packed_slots = 0;
+    bool lone = false;       // a slot is one wave's, not a workgroup's
 };
 
 SharedPlan shared_plan(const tt_decode_seq& prefix, const tt_decode_seq* seqs, int nseq, int Hq, int Hkv, int D, int kgs,

@@ -38,6 +38,12 @@
 namespace tt {
 namespace {
 
+// Rows of a KV head that a wave can take alone, and the tiles per CU (of all heads) from which on each wave takes tiles of its
+// own, four or more (whole call, a group's tiles | a wave's: 8 sequences, 32/32 heads of 80 behind 4k 37.1 | 29.8 us, behind
+// 16k 86.0 | 55.6, behind 2k 29.0 | 30.7; 32/32 heads of 128 behind 4k 43.1 | 38.4; 32/8 behind 8k 39.4 | 40.8, behind 16k
+// 46.6 | 46.0, behind 64k 92 | 76; slots of two tiles cost 12/4 heads of 96 behind 16k 40.5 instead of 34.2).
+constexpr int kLoneRows = 32;
+constexpr int kLoneTiles = 12;
 constexpr double kDenseCost = 1.5;  // an FP32 tile in packed ones
 
 // What the two ways to attend to a prefix take, in us, to choose between them. Multiplied for all sequences, a fixed part
@@ -238,6 +244,160 @@ __device__ __forceinline__ void pin(mf_u4& x, const int e) {
 
 // Ends a group of instructions that the scheduler may not mix with the next.
 __device__ __forceinline__ void slot_end() { __builtin_amdgcn_sched_barrier(0); }
+
+// Row n of a wave's 32, the lane's half h of each 16 channels.
+struct Row {
+    bool live;
+    int seq, head;
+};
+__device__ __forceinline__ Row row_of(const SharedArgs& a, const int kvh, const int rn, const int rows) {
+    const int G = a.Hq / a.Hkv;
+    const bool live = rn < rows;
+    return Row{live, live ? rn / G : 0, kvh * G + (live ? rn % G : 0)};
+}
+
+// Q' = Q 2^(12 - e), e the exponent of the row's largest value, in parts: channels 16 s + 8 h .. + 7. Returns the log2 units per
+// unit of the product.
+template <int ST>
+__device__ __forceinline__ float queries(const SharedArgs& a, const Row& row, const int h, const float neg1, mf_u4 (&qh)[ST],
+                                         mf_u4 (&ql)[ST]) {
+    const int D = a.D;
+    const float* q = global_ptr(a.seqs[row.seq].Q) + static_cast<size_t>(row.head) * D;
+    float mx = 0.0f;
+#pragma unroll
+    for (int s = 0; s < ST; ++s) {
+        const int c = min(16 * s + 8 * h, D - 8);
+        qh[s] = *reinterpret_cast<const un_u4*>(q + c);
+        ql[s] = *reinterpret_cast<const un_u4*>(q + c + 4);
+    }
+#pragma unroll
+    for (int s = 0; s < ST; ++s)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if (!row.live || 16 * s + 8 * h >= D) qh[s][j] = ql[s][j] = 0u;
+            mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(qh[s][j])), fabsf(__uint_as_float(ql[s][j]))));
+        }
+    const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+    mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+    const int e = (mx > 0.0f) ? __builtin_amdgcn_frexp_expf(mx) : 0;
+#pragma unroll
+    for (int s = 0; s < ST; ++s) {
+        uint2 p[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const mf_u4 x = j < 2 ? qh[s] : ql[s];
+            p[j] = tt::parts(__builtin_amdgcn_ldexpf(__uint_as_float(x[2 * (j & 1)]), 12 - e),
+                         __builtin_amdgcn_ldexpf(__uint_as_float(x[2 * (j & 1) + 1]), 12 - e), neg1);
+        }
+        qh[s] = mf_u4{p[0].x, p[1].x, p[2].x, p[3].x};
+        ql[s] = mf_u4{p[0].y, p[1].y, p[2].y, p[3].y};
+    }
+    return __builtin_amdgcn_ldexpf(a.scale2, e - 16);
+}
+
+// The softmax of a tile's logits d (lane (h, n): tokens 8 (r / 4) + 4 h + r % 4 of row n; `mask` its attended tokens, c log2 units per
+// unit, `meta` packed V's scales and zeros) into P, times V's scale where that is packed, in parts as the PV A operand.
+struct Soft {
+    float mr = -3.0e38f, l = 0.0f, pz = 0.0f;  // reference, sum, sum of P times the centred zero
+};
+template <int DC, bool PACKED, typename F>
+__device__ __forceinline__ void softmax32(Soft& s_, mf_f16& d, mf_f16 (&acc)[DC], const uint32_t mask, const float c, const char* meta,
+                                          const int lane, const float neg1, mf_u4 (&ph)[2], mf_u4 (&pl)[2], F&& before) {
+    float &mr = s_.mr, &l = s_.l, &pz = s_.pz;
+    const int h = lane >> 5;
+    auto now = [](int x) {
+        asm volatile("" : "+v"(x));
+        return x;
+    };
+    if (mask != 0xffffffffu) {
+        const uint32_t mine = mask >> (4 * (now(lane) >> 5));
+#pragma unroll
+        for (int r = 0; r < 16; ++r) d[r] = ((mine >> (8 * (r >> 2) + (r & 3))) & 1u) ? d[r] : kNegInf;
+    }
+    float mx = max3(max3(d[0], d[1], d[2]), max3(d[3], d[4], d[5]), max3(d[6], d[7], d[8]));
+    mx = max3(mx, max3(d[9], d[10], d[11]), max3(d[12], d[13], max3(d[14], d[15], d[15])));
+    mx = __builtin_fmaf(mx, c, -kUp);
+    // the reference moves only when a row's maximum passes it by more than the slack
+    if (__ballot(mx > mr + kSlack)) {
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
+        mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
+        const bool up = mx > mr + kSlack;
+        const float mn = up ? mx : mr;
+        const float al = up ? __builtin_amdgcn_exp2f(mr - mn) : 1.0f;
+        l *= al;
+        pz *= al;
+        const int from = 16 * (now(lane) >> 5);  // bytes: the lane group's first row
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float ar = __int_as_float(__builtin_amdgcn_ds_bpermute(from + 4 * (8 * (r >> 2) + (r & 3)), __float_as_int(al)));
+#pragma unroll
+            for (int s = 0; s < DC; ++s) acc[s][r] *= ar;
+        }
+        mr = mn;
+    }
+    before();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+        mf_f4 vs, vz;
+        if constexpr (PACKED) {
+            vs = *reinterpret_cast<const mf_f4*>(meta + 32 * j + 16 * h);
+            vz = *reinterpret_cast<const mf_f4*>(meta + 128 + 32 * j + 16 * h);
+        }
+        float p[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(d[4 * j + r], c, -mr));
+        l += (p[0] + p[1]) + (p[2] + p[3]);
+        if constexpr (PACKED) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                pz = __builtin_fmaf(p[r], vz[r], pz);
+                p[r] *= vs[r];
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 2; ++x) {
+            const uint2 y = tt::parts(p[2 * x], p[2 * x + 1], neg1);
+            ph[j >> 1][2 * (j & 1) + x] = y.x;
+            pl[j >> 1][2 * (j & 1) + x] = y.y;
+        }
+    }
+}
+
+// Writes a wave's partial, of rows row0 .. + 31. (NC: packed V's codes are 4^(c % NC) times too large.)
+template <int DC, int NC, bool PACKED>
+__device__ __forceinline__ void store32(const SharedArgs& a, const Row& row, const Soft& s_, const mf_f16 (&acc)[DC], const int v_exp,
+                                        const int lane, const int row0, const int rows, const int slot) {
+    const int D = a.D, n = lane & 31, h = lane >> 5;
+    // The partial in units of V: acc holds 16 V 2^-v_exp (FP32 tiles), or 2 4^(c % NC) of it without the centred zero.
+    auto both = [&](const float x) {  // a row's sum over its two lanes
+        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    };
+    const float l = both(s_.l);
+    const float z = PACKED ? __builtin_amdgcn_ldexpf(both(s_.pz), v_exp) : 0.0f;
+    const float back = __builtin_amdgcn_ldexpf(1.0f, v_exp - (PACKED ? 1 + 2 * (n & (NC - 1)) : 4));
+    // row n's partial, behind its sequence's own slots
+    const int ns = a.slot_base[row.seq + 1] - a.slot_base[row.seq];
+    const uint32_t pi = static_cast<uint32_t>(a.slot_base[row.seq] * a.Hq + row.head * ns + (ns - a.prefix_slots + slot));
+    if (h == 0 && row.live) {
+        a.ml[2 * static_cast<size_t>(pi)] = l > 0.0f ? s_.mr : kNegInf;
+        a.ml[2 * static_cast<size_t>(pi) + 1] = l;
+    }
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    const int first = 4 * (ln >> 5);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const int r_ = 8 * (r >> 2) + first + (r & 3);
+        const float zr = PACKED ? __shfl(z, r_, 64) : 0.0f;
+        const uint32_t pr = static_cast<uint32_t>(__shfl(static_cast<int>(pi), r_, 64));
+        if (row0 + r_ >= rows) continue;
+        float* o = a.acc + static_cast<size_t>(pr) * D + n;
+#pragma unroll
+        for (int s = 0; s < DC; ++s)
+            if (32 * s + n < D) o[32 * s] = __builtin_fmaf(acc[s][r], back, zr);
+    }
+}
 
 // One workgroup's share [t0, t1) of the prefix's tiles of one kind, for rows row0 .. of one KV head, head_dim up to
 // 32 DC. WM waves of 32 rows each, on the same tile.
@@ -495,50 +655,13 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
         }
         top = group_max<WM>(kmx, vmx, lds, wave, lane);
     }
-    // Q' = Q 2^(12 - e), e the exponent of the row's largest value: row n, channels 16 s + 8 h .. + 7.
-    const int rn = row0 + 32 * wave + n;
+    const Row row = row_of(a, kvh, row0 + 32 * wave + n, rows);
     const bool rowed = row0 + 32 * wave < rows;  // a wave without rows only stages (and multiplies zeros with K)
-    const bool live = rn < rows;
-    const int seq = live ? rn / G : 0;
-    const int head = kvh * G + (live ? rn % G : 0);
     mf_u4 qh[ST], ql[ST];
-    float crow;  // log2 units per unit of the product
-    {
-        const float* q = global_ptr(a.seqs[seq].Q) + static_cast<size_t>(head) * D;
-        float mx = 0.0f;
-#pragma unroll
-        for (int s = 0; s < ST; ++s) {
-            const int c = min(16 * s + 8 * h, D - 8);
-            qh[s] = *reinterpret_cast<const un_u4*>(q + c);
-            ql[s] = *reinterpret_cast<const un_u4*>(q + c + 4);
-        }
-#pragma unroll
-        for (int s = 0; s < ST; ++s)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                if (!live || 16 * s + 8 * h >= D) qh[s][j] = ql[s][j] = 0u;
-                mx = fmaxf(mx, fmaxf(fabsf(__uint_as_float(qh[s][j])), fabsf(__uint_as_float(ql[s][j]))));
-            }
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-        mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-        const int e = (mx > 0.0f) ? __builtin_amdgcn_frexp_expf(mx) : 0;
-#pragma unroll
-        for (int s = 0; s < ST; ++s) {
-            uint2 p[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const mf_u4 x = j < 2 ? qh[s] : ql[s];
-                p[j] = parts(__builtin_amdgcn_ldexpf(__uint_as_float(x[2 * (j & 1)]), 12 - e),
-                             __builtin_amdgcn_ldexpf(__uint_as_float(x[2 * (j & 1) + 1]), 12 - e));
-            }
-            qh[s] = mf_u4{p[0].x, p[1].x, p[2].x, p[3].x};
-            ql[s] = mf_u4{p[0].y, p[1].y, p[2].y, p[3].y};
-        }
-        crow = __builtin_amdgcn_ldexpf(a.scale2, e - 16);
-    }
+    const float crow = queries<ST>(a, row, h, neg1, qh, ql);
 
     mf_f16 acc[DC];
-    float mr = -3.0e38f, l = 0.0f, pz = 0.0f;
+    Soft st;
 #pragma unroll
     for (int s = 0; s < DC; ++s)
 #pragma unroll
@@ -628,7 +751,7 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
             }
             if (kn != k_exp || vn != v_exp) {
                 const float f = __builtin_amdgcn_ldexpf(1.0f, v_exp - vn);
-                pz *= f;
+                st.pz *= f;
 #pragma unroll
                 for (int s = 0; s < DC; ++s) acc[s] *= f;
                 k_exp = kn;
@@ -647,61 +770,9 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
                 vh[s & 1] = *reinterpret_cast<const mf_u4*>(x + L::V);
                 if constexpr (!PACKED) vw[s & 1] = *reinterpret_cast<const mf_u4*>(x + L::VLO);
             };
-            // Softmax: P (packed: P times V's scale) as the PV A operand.
-            if (mask != 0xffffffffu) {
-                const uint32_t mine = mask >> (4 * (now(lane) >> 5));
-#pragma unroll
-                for (int r = 0; r < 16; ++r) d[r] = ((mine >> (8 * (r >> 2) + (r & 3))) & 1u) ? d[r] : kNegInf;
-            }
-            const float c = __builtin_amdgcn_ldexpf(crow, k_exp);
-            float mx = max3(max3(d[0], d[1], d[2]), max3(d[3], d[4], d[5]), max3(d[6], d[7], d[8]));
-            mx = max3(mx, max3(d[9], d[10], d[11]), max3(d[12], d[13], max3(d[14], d[15], d[15])));
-            mx = __builtin_fmaf(mx, c, -kUp);
-            // the reference moves only when a row's maximum passes it by more than the slack
-            if (__ballot(mx > mr + kSlack)) {
-                const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(mx), __float_as_uint(mx), false, false);
-                mx = fmaxf(__uint_as_float(sw[0]), __uint_as_float(sw[1]));
-                const bool up = mx > mr + kSlack;
-                const float mn = up ? mx : mr;
-                const float al = up ? __builtin_amdgcn_exp2f(mr - mn) : 1.0f;
-                l *= al;
-                pz *= al;
-                const int from = 16 * (now(lane) >> 5);  // bytes: the lane group's first row
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const float ar = __int_as_float(__builtin_amdgcn_ds_bpermute(from + 4 * (8 * (r >> 2) + (r & 3)), __float_as_int(al)));
-#pragma unroll
-                    for (int s = 0; s < DC; ++s) acc[s][r] *= ar;
-                }
-                mr = mn;
-            }
             mf_u4 ph[2], pl[2];
-            load_v(0);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                mf_f4 vs, vz;
-                if constexpr (PACKED) {
-                    vs = *reinterpret_cast<const mf_f4*>(tl + L::VMETA + 32 * j + 16 * h);
-                    vz = *reinterpret_cast<const mf_f4*>(tl + L::VMETA + 128 + 32 * j + 16 * h);
-                }
-                float p[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) p[r] = __builtin_amdgcn_exp2f(__builtin_fmaf(d[4 * j + r], c, -mr));
-                l += (p[0] + p[1]) + (p[2] + p[3]);
-                if constexpr (PACKED) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        pz = __builtin_fmaf(p[r], vz[r], pz);
-                        p[r] *= vs[r];
-                    }
-                }
-#pragma unroll
-                for (int x = 0; x < 2; ++x) {
-                    const uint2 y = parts(p[2 * x], p[2 * x + 1]);
-                    ph[j >> 1][2 * (j & 1) + x] = y.x;
-                    pl[j >> 1][2 * (j & 1) + x] = y.y;
-                }
-            }
+            softmax32<DC, PACKED>(st, d, acc, mask, __builtin_amdgcn_ldexpf(crow, k_exp), tl + L::VMETA, lane, neg1, ph, pl,
+                                  [&]() { load_v(0); });
             constexpr int PR = PACKED ? 2 : 3, SLOTS = 2 * DC * PR;
             slot_end();
 #pragma unroll
@@ -716,33 +787,279 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
         k += skip | again ? 0 : 1;
     } while (k < t1);
 
-    // The partial in units of V: acc holds 16 V 2^-v_exp (FP32 tiles), or 2 4^(c % NC) of it without the centred zero.
-    auto both = [&](const float x) {  // a row's sum over its two lanes
-        const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        return __uint_as_float(sw[0]) + __uint_as_float(sw[1]);
+    store32<DC, NC, PACKED>(a, row, st, acc, v_exp, lane, row0 + 32 * wave, rows, slot);
+}
+
+// One wave's share of the tiles for at most 32 rows of one KV head, where there are no rows for more waves: each stages
+// whole tiles of its own, without a barrier, in its own part of the LDS. K of a tile is staged between the PV instructions
+// of the one before, V between its own QK ones, so that one buffer does. Scales change before a tile is staged. One wave per
+// SIMD, with up to 400 registers: the VALU, which unpacks a tile for 32 rows only, takes more of it than the matrix cores (8
+// sequences behind 16k tokens, 32/32 heads of 80: 16 to 17 tiles per wave, 56 us in all).
+template <int DC, bool PACKED, typename MetaT>
+__device__ __forceinline__ void lone_body(const SharedArgs& a, char* lds, const Tiers& t, const int kvh, const int row0,
+                                          const int rows, const int t0, const int t1, const int slot) {
+    using L = TileLds<DC>;
+    constexpr bool F16M = sizeof(MetaT) == 2;
+    constexpr int ST = 2 * DC;
+    float neg1 = -1.0f;
+    asm("" : "+s"(neg1));
+    auto parts = [&](const float x0, const float x1) { return tt::parts(x0, x1, neg1); };
+    const int lane = threadIdx.x & 63, n = lane & 31, h = lane >> 5;
+    const int D = a.D;
+    const uint32_t stride = static_cast<uint32_t>(a.Hkv) * D;
+    const int ktq = lane >> 3, kcq = lane & 7, vtq = lane & 7, vcq = lane >> 3;  // as for the larger groups, unit u: channels 32 u ..
+    const int total = PACKED ? t.slots : t.nd;
+    auto start_of = [&](const int tile) { return max(min(kTile * tile, total - kTile), 0); };
+    const int last = min(total, kTile) - 1;
+
+    uint32_t kx[DC][PACKED ? 12 : 16], vx[DC][PACKED ? 4 : 16], vm = 0u;
+    uint2 idv = make_uint2(0u, 0u);
+    auto get4 = [&](uint32_t* to, const void* base, const uint32_t off) {
+        const un_u4 y = load_at<un_u4>(base, off);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) to[e] = y[e];
     };
-    l = both(l);
-    const float z = PACKED ? __builtin_amdgcn_ldexpf(both(pz), v_exp) : 0.0f;
-    const float back = __builtin_amdgcn_ldexpf(1.0f, v_exp - (PACKED ? 1 + 2 * (n & (NC - 1)) : 4));
-    // row n's partial, behind its sequence's own slots
-    const int ns = a.slot_base[seq + 1] - a.slot_base[seq];
-    const uint32_t pi = static_cast<uint32_t>(a.slot_base[seq] * a.Hq + head * ns + (ns - a.prefix_slots + slot));
-    if (h == 0 && live) {
-        a.ml[2 * static_cast<size_t>(pi)] = l > 0.0f ? mr : kNegInf;
-        a.ml[2 * static_cast<size_t>(pi) + 1] = l;
-    }
-    const int first = 4 * (now(lane) >> 5);
+    auto fetch_k = [&](const int tile) {
+        const int s0 = start_of(tile);
+        constexpr uint32_t M = sizeof(MetaT);
+        if constexpr (PACKED) idv = load_at<uint2>(t.ids + s0, 8u * min(n, last));
 #pragma unroll
-    for (int r = 0; r < 16; ++r) {
-        const int row = 8 * (r >> 2) + first + (r & 3);
-        const float zr = PACKED ? __shfl(z, row, 64) : 0.0f;
-        const uint32_t pr = static_cast<uint32_t>(__shfl(static_cast<int>(pi), row, 64));
-        if (row0 + 32 * wave + row >= rows) continue;
-        float* o = a.acc + static_cast<size_t>(pr) * D + n;
+        for (int u = 0; u < DC; ++u) {
+            const uint32_t ck = min(32 * u + 4 * kcq, D - 4);
+            if constexpr (PACKED) {
+                const uint32_t kw = (min(4 * ktq, last) >> 4) * stride + ck, km = M * (a.kgs == 32 ? ck : kw);
+                const size_t kb = static_cast<size_t>(a.kgs == 32 ? s0 >> 5 : s0 >> 4) * stride * M;
+                get4(kx[u], t.kp + static_cast<size_t>(s0 >> 4) * stride, 4u * kw);
+                if constexpr (!F16M) {
+                    get4(kx[u] + 4, t.ks + kb, km);
+                    get4(kx[u] + 8, t.kz + kb, km);
+                } else {
+                    const un_u2 ps = load_at<un_u2>(t.ks + kb, km), pz = load_at<un_u2>(t.kz + kb, km);
+                    kx[u][4] = ps[0];
+                    kx[u][5] = ps[1];
+                    kx[u][6] = pz[0];
+                    kx[u][7] = pz[1];
+                }
+            } else {
 #pragma unroll
-        for (int s = 0; s < DC; ++s)
-            if (32 * s + n < D) o[32 * s] = __builtin_fmaf(acc[s][r], back, zr);
+                for (int j = 0; j < 4; ++j)
+                    get4(kx[u] + 4 * j, t.dk + static_cast<size_t>(s0) * stride, 4u * (min(4 * ktq + j, last) * stride + ck));
+            }
+        }
+    };
+    auto fetch_v = [&](const int tile) {
+        const int s0 = start_of(tile);
+        constexpr uint32_t M = sizeof(MetaT);
+        if constexpr (PACKED) {
+            const char* from = (lane < 32 ? t.vs : t.vz) + static_cast<size_t>(s0) * a.Hkv * M;
+            vm = load_at<MetaBits<MetaT>>(from, static_cast<uint32_t>(min(n, last)) * a.Hkv * M);
+        }
+#pragma unroll
+        for (int u = 0; u < DC; ++u) {
+            const uint32_t cv = min(32 * u + 4 * vcq, D - 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                if constexpr (PACKED)
+                    vx[u][j] = load_at<uint32_t>(t.vp + static_cast<size_t>(s0) * (stride / 16),
+                                                 4u * (min(4 * vtq + j, last) * (stride / 16) + (cv >> 4)));
+                else
+                    get4(vx[u] + 4 * j, t.dv + static_cast<size_t>(s0) * stride, 4u * (min(4 * vtq + j, last) * stride + cv));
+            }
+        }
+    };
+    auto mask_of = [&](const int tile) -> uint32_t {
+        const uint32_t in = total < kTile ? (1u << total) - 1u : 0xffffffffu << (kTile * tile - start_of(tile));
+        if constexpr (PACKED) return static_cast<uint32_t>(__ballot((idv.x & idv.y) != 0xffffffffu)) & in;
+        return in;
+    };
+
+    int k_exp = 0, v_exp = 0;
+    bool kfirst = true, vfirst = true;
+    Soft st;
+    mf_f16 acc[DC];
+#pragma unroll
+    for (int s = 0; s < DC; ++s)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) acc[s][r] = 0.0f;
+
+    // K's scales and zeros of the fetched tile (packed), and its exponent: what passes the limit, or comes first, sets it.
+    float ksc[PACKED ? DC : 1][4], kzr[PACKED ? DC : 1][4];
+    auto ready_k = [&](const uint32_t mask) {
+        float mx = 0.0f;
+#pragma unroll
+        for (int u = 0; u < DC; ++u) {
+            const int kc = 32 * u + 4 * kcq;
+            if constexpr (PACKED) {
+                const bool any = ((mask >> (4 * ktq)) & 15u) != 0u && kc < D;  // else they may be anything
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const uint32_t hs = kx[u][4 + (F16M ? e >> 1 : e)], hz = kx[u][F16M ? 6 + (e >> 1) : 8 + e];
+                    const float sc = F16M ? ((e & 1) ? half_hi(hs) : half_lo(hs)) : __uint_as_float(hs);
+                    const float zr = F16M ? ((e & 1) ? half_hi(hz) : half_lo(hz)) : __uint_as_float(hz);
+                    ksc[u][e] = any ? sc : 0.0f;
+                    kzr[u][e] = any ? zr : 0.0f;
+                    mx = fmaxf(mx, fmaxf(fabsf(kzr[u][e]), fabsf(__builtin_fmaf(3.0f, ksc[u][e], kzr[u][e]))));
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    mx = fmaxf(mx, ((mask >> (4 * ktq + i / 4)) & 1u) && kc < D ? fabsf(__uint_as_float(kx[u][i])) : 0.0f);
+            }
+        }
+        if (__ballot(__builtin_amdgcn_ldexpf(mx, 4 - k_exp) >= kLimit || (kfirst && mx > 0.0f))) {
+            k_exp = exponent(wave_max(mx), 8);
+            kfirst = false;
+        }
+        if constexpr (PACKED) {
+            const float by = __builtin_amdgcn_ldexpf(16.0f, -k_exp);
+#pragma unroll
+            for (int u = 0; u < DC; ++u)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    ksc[u][e] *= by;
+                    kzr[u][e] *= by;
+                }
+        }
+    };
+    auto k_token = [&](const int u, const int j, const uint32_t mask) {
+        const int kc = 32 * u + 4 * kcq;
+        float x[4];
+        if constexpr (PACKED) {
+            const uint32_t b = 0x0c0c0400u + 0x0101u * (ktq & 3);
+            const uint32_t codes = __builtin_amdgcn_perm(kx[u][1], kx[u][0], b) | (__builtin_amdgcn_perm(kx[u][3], kx[u][2], b) << 16);
+            uint32_t y = (codes >> (2 * j)) & 0x03030303u;
+            asm("" : "+v"(y));  // (or every code is extracted by an instruction of its own)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = __builtin_fmaf(static_cast<float>((y >> (8 * e)) & 0xffu), ksc[u][e], kzr[u][e]);
+        } else {
+            const bool in = ((mask >> (4 * ktq + j)) & 1u) && kc < D;
+            const float by = __builtin_amdgcn_ldexpf(16.0f, -k_exp);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = in ? __uint_as_float(kx[u][4 * j + e]) * by : 0.0f;
+        }
+        const uint2 p = parts(x[0], x[1]), q = parts(x[2], x[3]);
+        char* d = lds + (4 * ktq + j) * L::KS + 2 * kc;
+        *reinterpret_cast<uint2*>(d + L::KHI) = make_uint2(p.x, q.x);
+        *reinterpret_cast<uint2*>(d + L::KLO) = make_uint2(p.y, q.y);
+    };
+    // V's exponent, likewise, and packed V's scales and zeros to LDS.
+    auto ready_v = [&](const uint32_t mask) {
+        float mx = 0.0f, x = 0.0f;
+        const bool in = (mask >> n) & 1u;
+        if constexpr (PACKED) {
+            x = F16M ? half_lo(vm) : __uint_as_float(vm);
+            mx = lane < 32 && in ? fabsf(x) : 0.0f;
+        } else {
+#pragma unroll
+            for (int u = 0; u < DC; ++u)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    mx = fmaxf(mx, ((mask >> (4 * vtq + i / 4)) & 1u) && 32 * u + 4 * vcq < D ? fabsf(__uint_as_float(vx[u][i])) : 0.0f);
+        }
+        // (packed: a scale up to 2 2^v_exp stays in reach, P <= 2^14)
+        const bool past = PACKED ? __builtin_amdgcn_ldexpf(mx, -v_exp) >= 2.0f : __builtin_amdgcn_ldexpf(mx, 4 - v_exp) >= kLimit;
+        if (__ballot(past || (vfirst && mx > 0.0f))) {
+            const int e = exponent(wave_max(mx), PACKED ? 0 : 8);
+            const float f = __builtin_amdgcn_ldexpf(1.0f, v_exp - e);
+            st.pz *= f;
+#pragma unroll
+            for (int s = 0; s < DC; ++s) acc[s] *= f;
+            v_exp = e;
+            vfirst = false;
+        }
+        if constexpr (PACKED) {
+            const auto sw = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+            const float y = lane < 32 ? x : __builtin_fmaf(1.5f, __uint_as_float(sw[0]), x);
+            reinterpret_cast<float*>(lds + L::VMETA)[lane] = in ? __builtin_amdgcn_ldexpf(y, -v_exp) : 0.0f;
+        }
+    };
+    auto v_channel = [&](const int u, const int k, const uint32_t mask) {
+        const int vc = 32 * u + 4 * vcq;
+        char* d = lds + (vc + k) * L::VS + 32 * (vtq >> 2) + 16 * (vtq & 1) + 8 * ((vtq >> 1) & 1);
+        if constexpr (PACKED) {
+            const uint32_t b = 0x0c040c00u + 0x00010001u * (vcq & 3), mk = 0x00060006u << (2 * k);
+            const uint32_t y0 = __builtin_amdgcn_perm(vx[u][1], vx[u][0], b) << 1, y1 = __builtin_amdgcn_perm(vx[u][3], vx[u][2], b) << 1;
+            const _Float16 c = static_cast<_Float16>(1024.0f + 3.0f * static_cast<float>(1 << (2 * k)));
+            const mf_h2 off = {c, c};
+            const mf_h2 z0 = __builtin_bit_cast(mf_h2, (y0 & mk) | 0x64006400u) - off;
+            const mf_h2 z1 = __builtin_bit_cast(mf_h2, (y1 & mk) | 0x64006400u) - off;
+            *reinterpret_cast<uint2*>(d + L::V) = make_uint2(__builtin_bit_cast(uint32_t, z0), __builtin_bit_cast(uint32_t, z1));
+        } else {
+            const float by = __builtin_amdgcn_ldexpf(16.0f, -v_exp);
+            float y[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                y[j] = ((mask >> (4 * vtq + j)) & 1u) && vc < D ? __uint_as_float(vx[u][4 * j + k]) * by : 0.0f;
+            const uint2 p = parts(y[0], y[1]), q = parts(y[2], y[3]);
+            *reinterpret_cast<uint2*>(d + L::V) = make_uint2(p.x, q.x);
+            *reinterpret_cast<uint2*>(d + L::VLO) = make_uint2(p.y, q.y);
+        }
+    };
+
+    fetch_k(t0);
+    fetch_v(t0);
+    const Row row = row_of(a, kvh, row0 + n, rows);
+    mf_u4 qh[ST], ql[ST];
+    const float crow = queries<ST>(a, row, h, neg1, qh, ql);
+    uint32_t mask = mask_of(t0);
+    ready_k(mask);
+#pragma unroll
+    for (int i = 0; i < 4 * DC; ++i) k_token(i / 4, i % 4, mask);
+    fetch_k(min(t0 + 1, t1 - 1));
+#pragma unroll 1
+    for (int k = t0; k < t1; ++k) {
+        ready_v(mask);
+        wave_lds_sync();
+        mf_f16 d;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) d[r] = 0.0f;
+        {
+            const char* kl = lds + n * L::KS + 16 * h;
+            mf_u4 kh[2], kw[2];
+            auto load_k = [&](const int s) {
+                kh[s & 1] = *reinterpret_cast<const mf_u4*>(kl + L::KHI + 32 * s);
+                kw[s & 1] = *reinterpret_cast<const mf_u4*>(kl + L::KLO + 32 * s);
+            };
+            constexpr int PIECES = 4 * DC, SLOTS = 3 * ST;
+            load_k(0);
+            slot_end();
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i) {
+                const int s = i / 3;
+                if (i % 3 == 0 && s + 1 < ST) load_k(s + 1);
+                d = mfma32x32x16(i % 3 == 2 ? kw[s & 1] : kh[s & 1], i % 3 == 0 ? ql[s] : qh[s], d);
+#pragma unroll
+                for (int o = i * PIECES / SLOTS; o < (i + 1) * PIECES / SLOTS; ++o) v_channel(o / 4, o % 4, mask);
+                slot_end();
+            }
+        }
+        fetch_v(min(k + 1, t1 - 1));
+        wave_lds_sync();
+        mf_u4 vh[2], vw[2], ph[2], pl[2];
+        auto load_v = [&](const int s) {
+            const char* x = lds + (32 * (s >> 1) + n) * L::VS + 32 * (s & 1) + 16 * h;
+            vh[s & 1] = *reinterpret_cast<const mf_u4*>(x + L::V);
+            if constexpr (!PACKED) vw[s & 1] = *reinterpret_cast<const mf_u4*>(x + L::VLO);
+        };
+        softmax32<DC, PACKED>(st, d, acc, mask, __builtin_amdgcn_ldexpf(crow, k_exp), lds + L::VMETA, lane, neg1, ph, pl,
+                              [&]() { load_v(0); });
+        mask = mask_of(min(k + 1, t1 - 1));
+        ready_k(mask);
+        constexpr int PR = PACKED ? 2 : 3, SLOTS = 2 * DC * PR, PIECES = 4 * DC;
+        slot_end();
+#pragma unroll
+        for (int i = 0; i < SLOTS; ++i) {
+            const int s = i / PR, q = i % PR;
+            if (q == 0 && s + 1 < 2 * DC) load_v(s + 1);
+            acc[s >> 1] = mfma32x32x16(q == 0 ? pl[s & 1] : ph[s & 1], !PACKED && q == 1 ? vw[s & 1] : vh[s & 1], acc[s >> 1]);
+#pragma unroll
+            for (int o = i * PIECES / SLOTS; o < (i + 1) * PIECES / SLOTS; ++o) k_token(o / 4, o % 4, mask);
+            slot_end();
+        }
+        fetch_k(min(k + 2, t1 - 1));
+        wave_lds_sync();
     }
+    store32<DC, 4, PACKED>(a, row, st, acc, v_exp, lane, row0, rows, slot);
 }
 
 // The same for head dims above 128, whose accumulators leave registers for 16 rows per wave. Eight waves,
@@ -1257,6 +1574,50 @@ attn_shared_kernel(const SharedArgs a) {
     }
 }
 
+// Waves with tiles of their own: four slots to a workgroup, those of all heads and chunks back to back on one XCD.
+template <int DC>
+struct Lone {
+    static constexpr int ROWS = kLoneRows;
+    static constexpr int LDS = 4 * TileLds<DC>::BYTES;
+};
+template <int DC, typename MetaT>
+__global__ void __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(1))) attn_shared_few_kernel(const SharedArgs a) {
+    __shared__ __align__(16) char lds[Lone<DC>::LDS];
+    const unsigned id = blockIdx.x;
+    const unsigned q = id >> 3;
+    const unsigned hc = static_cast<unsigned>(a.Hkv * a.chunks);
+    const int hz = static_cast<int>(q % hc);
+    const int wave = scalar(static_cast<int>(threadIdx.x) >> 6);
+    const int s = 4 * static_cast<int>((q / hc) * 8 + (id & 7)) + wave;
+    if (s >= a.prefix_slots) return;
+    const int kvh = hz / a.chunks, chunk = hz - kvh * a.chunks;
+    const int rows = a.nseq * (a.Hq / a.Hkv), row0 = chunk * Lone<DC>::ROWS;
+    const Tiers t = tiers_of(a, kvh);
+    char* own = lds + wave * TileLds<DC>::BYTES;
+    if (s < a.packed_slots) {
+        const int tiles = (t.slots + kTile - 1) / kTile;
+        lone_body<DC, true, MetaT>(a, own, t, kvh, row0, rows, share(tiles, s, a.packed_slots), share(tiles, s + 1, a.packed_slots), s);
+    } else {
+        const int tiles = (t.nd + kTile - 1) / kTile, nd = a.prefix_slots - a.packed_slots;
+        lone_body<DC, false, MetaT>(a, own, t, kvh, row0, rows, share(tiles, s - a.packed_slots, nd),
+                                    share(tiles, s - a.packed_slots + 1, nd), s);
+    }
+}
+
+template <int DC>
+int launch_few(SharedArgs a, const int rows, hipStream_t st) {
+    a.chunks = (rows + Lone<DC>::ROWS - 1) / Lone<DC>::ROWS;
+    const long long wgs = static_cast<long long>((a.prefix_slots + 31) / 32) * 8 * a.Hkv * a.chunks;
+    if (wgs > 0x00ffffffLL) TT_FAIL(TT_ERR_INVALID_ARGUMENT, "attention grid too large");
+    const dim3 grid(static_cast<unsigned>(wgs));
+    if (a.meta_fp16)
+        hipLaunchKernelGGL((attn_shared_few_kernel<DC, uint16_t>), grid, dim3(256), 0, st, a);
+    else
+        hipLaunchKernelGGL((attn_shared_few_kernel<DC, float>), grid, dim3(256), 0, st, a);
+    TT_LAUNCH_CHECK();
+    return TT_OK;
+}
+
 template <int DC, int WM>
 int launch(SharedArgs a, const int rows, hipStream_t st) {
     a.chunks = (rows + Config<DC, WM>::ROWS - 1) / Config<DC, WM>::ROWS;
@@ -1290,12 +1651,13 @@ auto for_shape(const int D, const int rows, F&& f) {
     return for_rows<kWideDC>(rows, f);
 }
 
-// Its rows per workgroup, and the workgroups that a CU holds.
+// The rows of a share of tiles, and the shares that a CU holds at a time.
 struct Shape {
     int rows, per_cu;
 };
-Shape shape_of(const int D, const int rows) {
-    return for_shape(D, rows, [](auto dc, auto wm) {
+Shape shape_of(const int D, const int rows, const bool lone) {
+    if (lone) return Shape{kLoneRows, 4};
+    return for_shape(D, rows, [&](auto dc, auto wm) {
         using C = Config<dc.value, wm.value>;
         return Shape{C::ROWS, C::PER_CU};
     });
@@ -1311,14 +1673,17 @@ SharedPlan shared_plan(const tt_decode_seq& prefix, const tt_decode_seq* seqs, i
     const long long dense = (static_cast<long long>(prefix.dense_count) + kTile - 1) / kTile;
     const long long packed = (static_cast<long long>(prefix.num_blocks) * kgs + kTile - 1) / kTile;
     const long long tokens = static_cast<long long>(prefix.dense_count) + static_cast<long long>(prefix.num_blocks) * kgs;
-    const Shape sh = shape_of(D, rows);
+    const double cost = packed + kDenseCost * dense;
+    p.lone = D <= 128 && rows <= kLoneRows && cost * Hkv >= 256 * kLoneTiles;
+    const Shape sh = shape_of(D, rows, p.lone);
     // One round of workgroups, each kind's share by what its tiles cost; fewer where another one's partials cost the merge
     // more than it saves the others in tiles (32 sequences behind 2k, 32/8 heads of 128: 41.9 -> 37.0 us).
     const long long groups = static_cast<long long>(Hkv) * ((rows + sh.rows - 1) / sh.rows);
-    const double cost = packed + kDenseCost * dense;
     const double merge = 8.0 * nseq * Hq * D / kMergeRate;  // us per slot
     const double best = std::sqrt(tile_us(D) * cost / merge);
-    const long long slots = std::max<long long>(1, std::min<long long>(256LL * sh.per_cu / groups, std::llround(best)));
+    long long slots = std::min<long long>(256LL * sh.per_cu / groups, std::llround(best));
+    if (p.lone) slots = std::min<long long>(slots, std::llround(cost / 4));
+    slots = std::max<long long>(1, slots);
     const double shared_us = kSharedUs + D / 16.0 + tile_us(D) * std::ceil(cost / slots) + merge * slots;
     p.per_seq = tokens > 0 && nseq <= kMaxBatchSeqs / 2 && walk_us(nseq, static_cast<double>(tokens), Hq, Hkv, D) <= shared_us ? 2 : 1;
     tt_decode_seq entries[kMaxBatchSeqs];
@@ -1369,6 +1734,8 @@ int shared_launch(const SharedPlan& plan, const tt_decode_seq& prefix, const tt_
         std::memcpy(a.slot_base, b.slot_base, sizeof(a.slot_base));
         const int rows = b.nseq * (Hq / Hkv);
         const int rc = for_shape(D, rows, [&](auto dc, auto wm) {
+            if constexpr (dc.value <= 4)
+                if (plan.lone) return launch_few<dc.value>(a, rows, stream);
             return launch<dc.value, wm.value>(a, rows, stream);
         });
         if (rc) return rc;
