@@ -425,7 +425,6 @@ __device__ __forceinline__ void shared_body(const SharedArgs& a, char* lds, cons
     const int lane = threadIdx.x & 63;
     const int wave = scalar(static_cast<int>(threadIdx.x) >> 6);
     const int n = lane & 31, h = lane >> 5;
-    const int G = a.Hq / a.Hkv;
     const int D = a.D;
     const uint32_t stride = static_cast<uint32_t>(a.Hkv) * D;  // elements between tokens (blocks) of a head
     // A unit is 64 lanes x (4 tokens x 4 channels) of a tile: 32 channels. Every wave stages the same share of a K and of
