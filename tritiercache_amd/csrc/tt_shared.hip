@@ -25,7 +25,7 @@
 // GHz), about as many the VALU's, which unpacks, exponentiates and splits P
 // (some 330 instructions per wave and tile of 32 tokens x 32 rows against 40
 // matrix ones), and the two hardly overlap with two waves per SIMD, the most
-// that 230 registers allow. Measured without gain: the two halves of the waves
+// that 250 registers allow. Measured without gain: the two halves of the waves
 // half a tile apart, K and V staged by different waves, priorities of the waves,
 // operands read two steps ahead.
 #include "tt_shared.h"
